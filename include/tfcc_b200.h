@@ -78,6 +78,9 @@ extern "C" {
 #define TFCCB200_DEV_TIMEOUT_MMA 0x2
 #define TFCCB200_DEV_TIMEOUT_CONVERT 0x4
 #define TFCCB200_DEV_TIMEOUT_EPILOGUE 0x8
+/* Bits of the cache kernels: device-resident indices that contradict the sizes the host gave. */
+#define TFCCB200_DEV_BAD_SEQUENCE 0x10 /* starts / lengths outside the packed rows, the table or the stated bounds */
+#define TFCCB200_DEV_BAD_PAGE 0x20     /* a table entry outside [0, pages) */
 
 TFCCB200_API const char* tfccb200_strerror(int status);
 
@@ -535,6 +538,101 @@ TFCCB200_API int tfccb200_qgemm_u8s8s32_host(void* stream, const uint8_t* hA, un
                                 float minB, float maxB, int32_t* hC, unsigned strideC,
                                 float* minC, float* maxC, unsigned M, unsigned N, unsigned K,
                                 unsigned batch);
+
+/*
+ * 8-bit linear layer with one scale per token and one per output channel (symmetric, no zero
+ * points): what the range-based quantized matmul above needs a minimum and maximum of the whole
+ * tensor for, these take row by row.
+ *
+ * tfccb200_quantize_tokens_f32: row r of src (cols floats, rows ld_src apart) becomes
+ *   scales[r] = fl32(max|x| / 127),  codes[r][c] = round_half_even(x / scales[r]) in [-127, 127]
+ * decided by the exact quotient.  A row of zeros gets scale 0 and codes 0; a row with an infinity
+ * or a NaN scale NaN and codes 0.  Rows of codes are ld_codes bytes apart, and the columns between cols
+ * and ld_codes are left as they are.
+ *
+ * tfccb200_qgemm_scaled_s8: C = act(a_scales[m] * b_scales[n] * (A.B)[m][n] + bias[n]), the int32
+ * sums exact for K <= 133,000; A [M,K] s8 with rows lda apart, B [K,N] s8 with rows ldb apart, C [M,N]
+ * fp32 dense, bias [N] or NULL.  Bases 16-byte aligned with lda and ldb multiples of 16 run on the tensor
+ * cores; any other layout on the CUDA cores.  TFCCB200_EUNSUPPORTED when a forced path cannot take
+ * the operands.
+ *
+ * tfccb200_qlinear_f32: both in one call: x [M,K] fp32 with rows ldx apart, the codes and scales of x
+ * in the caller's workspace (tfccb200_qlinear_workspace bytes, 256-byte aligned).
+ * No counterpart in the reference, whose quantized matmul is the range-based one.
+ */
+TFCCB200_API int tfccb200_quantize_tokens_f32(void* stream, const float* src, size_t ld_src,
+                                              unsigned rows, unsigned cols, int8_t* codes,
+                                              size_t ld_codes, float* scales);
+TFCCB200_API int tfccb200_qgemm_scaled_s8(void* stream, const int8_t* A, size_t lda,
+                                          const float* a_scales, const int8_t* B, size_t ldb,
+                                          const float* b_scales, const float* bias, float* C,
+                                          unsigned M, unsigned N, unsigned K, int activation,
+                                          int path, int* device_status);
+TFCCB200_API int tfccb200_qlinear_f32(void* stream, const float* x, size_t ldx, const int8_t* B,
+                                      size_t ldb, const float* b_scales, const float* bias,
+                                      float* C, unsigned M, unsigned N, unsigned K, int activation,
+                                      void* workspace, size_t workspace_bytes, int* device_status);
+TFCCB200_API size_t tfccb200_qlinear_workspace(unsigned M, unsigned K);
+
+/*
+ * Paged 8-bit key / value cache.  The pool lies in the caller's memory: codes
+ * [pages, kv_heads, page_size, dim] s8 and scales [pages, kv_heads, page_size] fp32, for keys and for
+ * values (k = scale * code).  dim 64 or 128, page_size a power of two up to 1024.
+ *
+ * The sequences of a call are device data: rows starts[b] .. starts[b+1] of the packed [rows, ...]
+ * tensors are the new tokens of sequence b (starts has batch + 1 entries), lengths[b] the tokens
+ * it has in the cache, the new ones included; position p lies in page
+ * table[b * table_width + p / page_size], slot p % page_size.  A kernel checks what it reads: a sequence
+ * whose rows leave [0, rows] or whose length exceeds table_width * page_size (or max_length) is
+ * passed over and TFCCB200_DEV_BAD_SEQUENCE raised; a page outside [0, pages) raises
+ * TFCCB200_DEV_BAD_PAGE: nothing is written to it, reading gives 0, and rows that attend to it are
+ * NaN.  Rows behind starts[batch] are left as they are.  New tokens beyond lengths[b]
+ * (a length smaller than the number of new tokens) have no position: they are not written, and
+ * read as 0.
+ *
+ * Pointers are 16-byte aligned, row pitches (ld*, in elements) multiples of 4 and at least
+ * heads * dim.
+ *
+ * tfccb200_cache_append_f32 quantizes k and v [rows, kv_heads * dim] as tfccb200_quantize_tokens_f32
+ * does, one scale per token and head, into their pages.  Two new tokens must not share a slot.
+ * tfccb200_cache_read_f32 is the inverse for the same tokens: scale * code.  With starts counting
+ * whole sequences (starts[b+1] - starts[b] == lengths[b]) it reads all of them.
+ * tfccb200_cache_attention_f32: out_i = sum_j softmax_j(scale * q_i.k_j) v_j for q and out
+ * [rows, heads * dim], query head h reading kv head h / (heads / kv_heads), j over the cached tokens
+ * of the row's sequence up to its own position (causal) or all of them; a row that sees none is
+ * 0.  max_new and max_length bound the new and cached tokens of one sequence; the launch is shaped
+ * by them, and a sequence that exceeds them is passed over with TFCCB200_DEV_BAD_SEQUENCE.
+ * workspace: tfccb200_cache_attention_workspace bytes, 256-byte aligned.
+ */
+typedef struct tfccb200_cache {
+  int8_t* keys;
+  float* key_scales;
+  int8_t* values;
+  float* value_scales;
+  unsigned pages, page_size, kv_heads, dim;
+} tfccb200_cache;
+TFCCB200_API int tfccb200_cache_append_f32(void* stream, const tfccb200_cache* cache,
+                                           const float* k, size_t ldk, const float* v, size_t ldv,
+                                           const int32_t* starts, const int32_t* lengths,
+                                           const int32_t* table, unsigned batch,
+                                           unsigned table_width, unsigned rows,
+                                           int* device_status);
+TFCCB200_API int tfccb200_cache_read_f32(void* stream, const tfccb200_cache* cache, float* k,
+                                         size_t ldk, float* v, size_t ldv, const int32_t* starts,
+                                         const int32_t* lengths, const int32_t* table,
+                                         unsigned batch, unsigned table_width, unsigned rows,
+                                         int* device_status);
+TFCCB200_API int tfccb200_cache_attention_f32(void* stream, const tfccb200_cache* cache,
+                                              const float* q, size_t ldq, float* out, size_t ldo,
+                                              const int32_t* starts, const int32_t* lengths,
+                                              const int32_t* table, unsigned batch,
+                                              unsigned table_width, unsigned rows, unsigned heads,
+                                              unsigned max_new, unsigned max_length, float scale,
+                                              int causal, void* workspace, size_t workspace_bytes,
+                                              int* device_status);
+TFCCB200_API size_t tfccb200_cache_attention_workspace(const tfccb200_cache* cache, unsigned batch,
+                                                       unsigned rows, unsigned heads,
+                                                       unsigned max_new, unsigned max_length);
 
 /*
  * Test hook for the give-up path of the fp32 tensor-core kernel.  CTAs that share a tile's

@@ -62,6 +62,15 @@ class _Lib:
             "tfccb200_quantize_rowsum_f32": (i, [vp, vp, u, u, vp, vp, vp, i, vp]),
             "tfccb200_dequantize_f32": (i, [vp, vp, i, sz, vp, vp, vp]),
             "tfccb200_requantize": (i, [vp, vp, i, sz, vp, vp, vp, vp, vp, i]),
+            "tfccb200_quantize_tokens_f32": (i, [vp, vp, sz, u, u, vp, sz, vp]),
+            "tfccb200_qgemm_scaled_s8": (i, [vp, vp, sz, vp, vp, sz, vp, vp, vp, u, u, u, i, i, vp]),
+            "tfccb200_qlinear_f32": (i, [vp, vp, sz, vp, sz, vp, vp, vp, u, u, u, i, vp, sz, vp]),
+            "tfccb200_qlinear_workspace": (sz, [u, u]),
+            "tfccb200_cache_append_f32": (i, [vp, vp, vp, sz, vp, sz, vp, vp, vp, u, u, u, vp]),
+            "tfccb200_cache_read_f32": (i, [vp, vp, vp, sz, vp, sz, vp, vp, vp, u, u, u, vp]),
+            "tfccb200_cache_attention_f32": (i, [vp, vp, vp, sz, vp, sz, vp, vp, vp, u, u, u, u, u, u,
+                                                 f, i, vp, sz, vp]),
+            "tfccb200_cache_attention_workspace": (sz, [vp, u, u, u, u, u]),
             "tfccb200_sgemm_nsplit_push": (i, [vp, vp, vp, C.POINTER(C.c_void_p), u, u, vp, u, u, u, i, vp, vp, C.c_size_t, vp]),
             "tfccb200_sgemm_nsplit_push_ex": (i, [vp, vp, vp, C.POINTER(C.c_void_p), u, u, vp, u, u, u, i, vp, vp, C.c_size_t, u, vp]),
             "tfccb200_qgemm_nsplit_push": (i, [vp, vp, vp, i32, vp, vp, i32, C.POINTER(C.c_void_p), u, u, u, u, u, vp, vp]),
@@ -111,6 +120,9 @@ EXPORTED_SYMBOLS = (
     "tfccb200_sgemm_act", "tfccb200_attention_f32", "tfccb200_softmax_f32", "tfccb200_layer_norm_f32", "tfccb200_gelu_f32",
     "tfccb200_permute_0213_f32", "tfccb200_transpose_last2_f32",
     "tfccb200_minmax_f32", "tfccb200_quantize_f32", "tfccb200_quantize_rowsum_f32", "tfccb200_dequantize_f32", "tfccb200_requantize",
+    "tfccb200_quantize_tokens_f32", "tfccb200_qgemm_scaled_s8", "tfccb200_qlinear_f32",
+    "tfccb200_qlinear_workspace", "tfccb200_cache_append_f32", "tfccb200_cache_read_f32",
+    "tfccb200_cache_attention_f32", "tfccb200_cache_attention_workspace",
     "tfccb200_sgemm_nsplit_push", "tfccb200_sgemm_nsplit_push_ex", "tfccb200_qgemm_nsplit_push",
     "tfccb200_sgemm_nsplit_host", "tfccb200_group_create", "tfccb200_group_destroy",
     "tfccb200_group_size", "tfccb200_group_device", "tfccb200_group_stream", "tfccb200_group_sync",

@@ -831,4 +831,165 @@ int tfccb200_qgemm_u8s8s32_host(void* stream, const uint8_t* hA, unsigned stride
   return dev_status ? TFCCB200_EDEVICE : TFCCB200_OK;
 }
 
+namespace {
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+int run_s8_gemm(const S8GemmArgs& a, int path) {
+  if (!a.A || !a.B || !a.C || !a.a_scales || !a.b_scales || a.M == 0 || a.N == 0 || a.K == 0)
+    return TFCCB200_EINVAL;
+  if (a.lda < a.K || a.ldb < a.N) return TFCCB200_EINVAL;
+  if (a.activation != TFCCB200_ACT_NONE && a.activation != TFCCB200_ACT_GELU_ERF) return TFCCB200_EINVAL;
+  if (a.K > 133000u) return TFCCB200_EOVERFLOW;  // 127 * 127 * K must fit an int32
+  if (shape_overflows(a.M, a.N, a.K, 1)) return TFCCB200_EOVERFLOW;
+  if (misaligned(a.C, 4) || misaligned(a.a_scales, 4) || misaligned(a.b_scales, 4) || misaligned(a.bias, 4))
+    return TFCCB200_EALIGN;
+  switch (path) {
+    case TFCCB200_PATH_AUTO: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, -1) : simt_s8_gemm(a);
+    case TFCCB200_PATH_SIMT: return simt_s8_gemm(a);
+    case TFCCB200_PATH_UMMA: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 0) : TFCCB200_EUNSUPPORTED;
+    case TFCCB200_PATH_UMMA2: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 1) : TFCCB200_EUNSUPPORTED;
+    default: return TFCCB200_EINVAL;
+  }
+}
+
+// Row pitch of the codes that tfccb200_qlinear_f32 keeps in the workspace.
+size_t code_pitch(unsigned K) { return (static_cast<size_t>(K) + 15) / 16 * 16; }
+
+int fill_cache(CacheArgs& a, void* stream, const tfccb200_cache* c, const int32_t* starts, const int32_t* lengths,
+               const int32_t* table, unsigned batch, unsigned table_width, unsigned rows, int* status) {
+  if (!c || !c->keys || !c->key_scales || !c->values || !c->value_scales || !starts || !lengths || !table)
+    return TFCCB200_EINVAL;
+  if (c->pages == 0 || c->kv_heads == 0 || batch == 0 || table_width == 0 || rows == 0) return TFCCB200_EINVAL;
+  if (c->dim != 64 && c->dim != 128) return TFCCB200_EUNSUPPORTED;
+  if (c->page_size == 0 || c->page_size > 1024 || (c->page_size & (c->page_size - 1))) return TFCCB200_EUNSUPPORTED;
+  if (misaligned(c->keys, 16) || misaligned(c->values, 16) || misaligned(c->key_scales, 4) ||
+      misaligned(c->value_scales, 4) || misaligned(starts, 4) || misaligned(lengths, 4) || misaligned(table, 4))
+    return TFCCB200_EALIGN;
+  // page numbers and positions are int32
+  if (c->pages > 0x7fffffffu || rows > 0x7fffffffu || c->kv_heads > 65535u || batch > (1u << 24) ||
+      static_cast<unsigned long long>(table_width) * c->page_size > 0x7fffff00ull)
+    return TFCCB200_EOVERFLOW;
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.keys = c->keys; a.key_scales = c->key_scales;
+  a.values = c->values; a.value_scales = c->value_scales;
+  a.pages = c->pages; a.page_size = c->page_size; a.kv_heads = c->kv_heads; a.dim = c->dim;
+  a.starts = starts; a.lengths = lengths; a.table = table;
+  a.batch = batch; a.table_width = table_width; a.rows = rows;
+  a.status = status;
+  return TFCCB200_OK;
+}
+
+int check_rows(const void* p, size_t ld, size_t width) {
+  if (!p || ld < width) return TFCCB200_EINVAL;
+  return misaligned(p, 16) || ld % 4 ? TFCCB200_EALIGN : TFCCB200_OK;
+}
+
+}  // namespace
+
+int tfccb200_quantize_tokens_f32(void* stream, const float* src, size_t ld_src, unsigned rows, unsigned cols,
+                                 int8_t* codes, size_t ld_codes, float* scales) {
+  if (!src || !codes || !scales || rows == 0 || cols == 0 || ld_src < cols || ld_codes < cols) return TFCCB200_EINVAL;
+  if (misaligned(src, 4) || misaligned(scales, 4)) return TFCCB200_EALIGN;
+  if (rows > 0x7fffffffu) return TFCCB200_EOVERFLOW;
+  return quantize_tokens(static_cast<cudaStream_t>(stream), src, ld_src, rows, cols, codes, ld_codes, scales);
+}
+
+int tfccb200_qgemm_scaled_s8(void* stream, const int8_t* A, size_t lda, const float* a_scales, const int8_t* B,
+                             size_t ldb, const float* b_scales, const float* bias, float* C, unsigned M, unsigned N,
+                             unsigned K, int activation, int path, int* device_status) {
+  S8GemmArgs a = {};
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.A = A; a.B = B; a.C = C;
+  a.a_scales = a_scales; a.b_scales = b_scales; a.bias = bias;
+  a.lda = lda; a.ldb = ldb;
+  a.M = M; a.N = N; a.K = K;
+  a.activation = activation;
+  a.status = device_status;
+  return run_s8_gemm(a, path);
+}
+
+size_t tfccb200_qlinear_workspace(unsigned M, unsigned K) {
+  return (static_cast<size_t>(M) * 4 + 255) / 256 * 256 + static_cast<size_t>(M) * code_pitch(K);
+}
+
+int tfccb200_qlinear_f32(void* stream, const float* x, size_t ldx, const int8_t* B, size_t ldb,
+                         const float* b_scales, const float* bias, float* C, unsigned M, unsigned N, unsigned K,
+                         int activation, void* workspace, size_t workspace_bytes, int* device_status) {
+  if (!x || M == 0 || K == 0 || ldx < K) return TFCCB200_EINVAL;
+  if (!workspace || misaligned(workspace, 256) || workspace_bytes < tfccb200_qlinear_workspace(M, K))
+    return TFCCB200_EWORKSPACE;
+  float* scales = static_cast<float*>(workspace);
+  S8GemmArgs a = {};
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.A = static_cast<int8_t*>(workspace) + (static_cast<size_t>(M) * 4 + 255) / 256 * 256;
+  a.B = B; a.C = C;
+  a.a_scales = scales; a.b_scales = b_scales; a.bias = bias;
+  a.lda = code_pitch(K); a.ldb = ldb;
+  a.M = M; a.N = N; a.K = K;
+  a.activation = activation;
+  a.status = device_status;
+  // everything run_s8_gemm would refuse is refused before the first launch
+  if (!B || !C || !b_scales || N == 0 || ldb < N) return TFCCB200_EINVAL;
+  if (activation != TFCCB200_ACT_NONE && activation != TFCCB200_ACT_GELU_ERF) return TFCCB200_EINVAL;
+  if (K > 133000u || shape_overflows(M, N, K, 1)) return TFCCB200_EOVERFLOW;
+  const int st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
+  return st != TFCCB200_OK ? st : run_s8_gemm(a, TFCCB200_PATH_AUTO);
+}
+
+int tfccb200_cache_append_f32(void* stream, const tfccb200_cache* cache, const float* k, size_t ldk, const float* v,
+                              size_t ldv, const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                              unsigned batch, unsigned table_width, unsigned rows, int* device_status) {
+  CacheArgs a = {};
+  int st = fill_cache(a, stream, cache, starts, lengths, table, batch, table_width, rows, device_status);
+  const size_t width = st == TFCCB200_OK ? static_cast<size_t>(a.kv_heads) * a.dim : 0;
+  if (st == TFCCB200_OK) st = check_rows(k, ldk, width);
+  if (st == TFCCB200_OK) st = check_rows(v, ldv, width);
+  return st != TFCCB200_OK ? st : cache_append(a, k, ldk, v, ldv);
+}
+
+int tfccb200_cache_read_f32(void* stream, const tfccb200_cache* cache, float* k, size_t ldk, float* v, size_t ldv,
+                            const int32_t* starts, const int32_t* lengths, const int32_t* table, unsigned batch,
+                            unsigned table_width, unsigned rows, int* device_status) {
+  CacheArgs a = {};
+  int st = fill_cache(a, stream, cache, starts, lengths, table, batch, table_width, rows, device_status);
+  const size_t width = st == TFCCB200_OK ? static_cast<size_t>(a.kv_heads) * a.dim : 0;
+  if (st == TFCCB200_OK) st = check_rows(k, ldk, width);
+  if (st == TFCCB200_OK) st = check_rows(v, ldv, width);
+  return st != TFCCB200_OK ? st : cache_read(a, k, ldk, v, ldv);
+}
+
+size_t tfccb200_cache_attention_workspace(const tfccb200_cache* cache, unsigned batch, unsigned rows, unsigned heads,
+                                          unsigned max_new, unsigned max_length) {
+  if (!cache || cache->kv_heads == 0 || heads % cache->kv_heads) return 0;
+  CacheAttentionArgs a = {};
+  a.cache.kv_heads = cache->kv_heads; a.cache.dim = cache->dim; a.cache.page_size = cache->page_size;
+  a.cache.batch = batch; a.cache.rows = rows;
+  a.heads = heads; a.max_new = max_new; a.max_length = max_length;
+  return cache_attention_workspace(a);
+}
+
+int tfccb200_cache_attention_f32(void* stream, const tfccb200_cache* cache, const float* q, size_t ldq, float* out,
+                                 size_t ldo, const int32_t* starts, const int32_t* lengths, const int32_t* table,
+                                 unsigned batch, unsigned table_width, unsigned rows, unsigned heads,
+                                 unsigned max_new, unsigned max_length, float scale, int causal, void* workspace,
+                                 size_t workspace_bytes, int* device_status) {
+  CacheAttentionArgs a = {};
+  int st = fill_cache(a.cache, stream, cache, starts, lengths, table, batch, table_width, rows, device_status);
+  if (st != TFCCB200_OK) return st;
+  if (heads == 0 || heads % a.cache.kv_heads || max_new == 0 || max_length == 0) return TFCCB200_EINVAL;
+  const size_t width = static_cast<size_t>(heads) * a.cache.dim;
+  if ((st = check_rows(q, ldq, width)) != TFCCB200_OK || (st = check_rows(out, ldo, width)) != TFCCB200_OK) return st;
+  if (static_cast<unsigned long long>(rows) * heads > 0x7fffffffull) return TFCCB200_EOVERFLOW;
+  a.q = q; a.out = out; a.ldq = ldq; a.ldo = ldo;
+  a.heads = heads;
+  a.max_new = max_new; a.max_length = max_length;
+  a.scale = scale;
+  a.causal = causal ? 1 : 0;
+  a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+  const size_t need = cache_attention_workspace(a);
+  if (need && (!workspace || misaligned(workspace, 256) || workspace_bytes < need)) return TFCCB200_EWORKSPACE;
+  return cache_attention(a);
+}
+
 }  // extern "C"

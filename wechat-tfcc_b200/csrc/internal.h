@@ -205,4 +205,58 @@ int requantize(cudaStream_t stream, const void* src, int src_type, size_t n, con
                const float* pmax_in, const float* pmin_out, const float* pmax_out, void* dst,
                int dst_type);
 
+// ---- 8-bit linear layer: a scale per token and per channel (s8_kernels.cu, umma_launch.cu) ----
+struct S8GemmArgs {
+  cudaStream_t stream;
+  const int8_t* A;  // [M, K], rows lda apart
+  const int8_t* B;  // [K, N], rows ldb apart
+  float* C;         // [M, N] dense
+  const float* a_scales;
+  const float* b_scales;
+  const float* bias;  // [N] or nullptr
+  unsigned long long lda, ldb;
+  unsigned M, N, K;
+  int activation;
+  int* status;
+};
+int quantize_tokens(cudaStream_t stream, const float* src, unsigned long long ld_src, unsigned rows,
+                    unsigned cols, int8_t* codes, unsigned long long ld_codes, float* scales);
+int simt_s8_gemm(const S8GemmArgs& a);
+bool umma_s8_gemm_supported(const S8GemmArgs& a);
+int umma_s8_gemm(const S8GemmArgs& a, int force_pair);  // force_pair: -1 = choose
+
+// ---- paged 8-bit cache (cache.cu, cache_attention.cu) ----
+struct CacheArgs {
+  cudaStream_t stream;
+  int8_t* keys;  // [pages, kv_heads, page_size, dim], scales without the last dimension
+  float* key_scales;
+  int8_t* values;
+  float* value_scales;
+  unsigned pages, page_size, kv_heads, dim;
+  const int32_t* starts;   // [batch + 1]
+  const int32_t* lengths;  // [batch]
+  const int32_t* table;    // [batch, table_width]
+  unsigned batch, table_width, rows;
+  int* status;
+};
+struct CacheParams;
+CacheParams cache_params(const CacheArgs& a);
+int cache_append(const CacheArgs& a, const float* k, unsigned long long ldk, const float* v,
+                 unsigned long long ldv);
+int cache_read(const CacheArgs& a, float* k, unsigned long long ldk, float* v, unsigned long long ldv);
+struct CacheAttentionArgs {
+  CacheArgs cache;
+  const float* q;
+  float* out;
+  unsigned long long ldq, ldo;
+  unsigned heads;
+  unsigned max_new, max_length;  // bounds the caller knows on the host
+  float scale;
+  int causal;
+  void* workspace;
+  size_t workspace_bytes;
+};
+size_t cache_attention_workspace(const CacheAttentionArgs& a);
+int cache_attention(const CacheAttentionArgs& a);
+
 }  // namespace tfccb200

@@ -275,7 +275,9 @@ __device__ __forceinline__ void tmem_ld_wait() {
 }
 
 // ---- tcgen05.mma ----------------------------------------------------------------
-enum class MmaKind { TF32, I8, BF16 };
+// I8: u8 x s8, S8: s8 x s8 (the same instruction kind, told apart by the instruction descriptor).
+enum class MmaKind { TF32, I8, BF16, S8 };
+__host__ __device__ constexpr bool is_8bit(MmaKind k) { return k == MmaKind::I8 || k == MmaKind::S8; }
 
 // D[tmem] (+)= A[smem] . B[smem]; `accumulate` == 0 overwrites D.
 template <MmaKind kKind, int kCtaGroup>
@@ -309,7 +311,7 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t 
         :
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
-  } else if constexpr (kKind == MmaKind::I8 && kCtaGroup == 1) {
+  } else if constexpr (is_8bit(kKind) && kCtaGroup == 1) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"

@@ -12,6 +12,8 @@
 //     fp32 GEMM.
 //   * I8: u8 x s8 -> s32, exact, with the zero-point correction applied while
 //     the accumulator leaves tensor memory.
+//   * S8: s8 x s8, the exact int32 sums times a scale per row and per column (+ bias, activation)
+//     as fp32.
 //   * BF16 on operands that a pre-pass rounded from fp32 to bfloat16 (opt-in
 //     low-precision mode); fp32 accumulation and fp32 output.
 //
@@ -80,6 +82,8 @@ struct UmmaGemmParams {
   unsigned col_offset;     // first destination column of this problem's column 0
   const float* bias;       // [N] or nullptr (float kinds only)
   int activation;          // TFCCB200_ACT_*, applied after the bias (float kinds only)
+  const float* a_scales;   // S8: scale of every row of A, [M]
+  const float* b_scales;   // S8: scale of every column of B, [N]
   const int32_t* rsA;      // I8: row sums of A, [batch?][M]
   const int32_t* rsB;      // I8: column sums of B, [batch?][N]
   int32_t offA, offB;      // I8 zero-point offsets
@@ -196,7 +200,7 @@ struct UmmaGemmConfig {
           ? ptx::make_idesc(1u, 2u, 2u, 0u, 1u, static_cast<uint32_t>(kTileM), BN)
           : (kKind == ptx::MmaKind::BF16)
                 ? ptx::make_idesc(1u, 1u, 1u, 0u, 1u, static_cast<uint32_t>(kTileM), BN)
-                : ptx::make_idesc(2u, 0u, 1u, 0u, 1u, static_cast<uint32_t>(kTileM), BN);
+                : ptx::make_idesc(2u, kKind == ptx::MmaKind::S8 ? 1u : 0u, 1u, 0u, 1u, static_cast<uint32_t>(kTileM), BN);
   static_assert(BN % 16 == 0 && BN >= 16 && BN <= 256, "MMA N out of range");
   static_assert((BN & (BN - 1)) == 0, "BN must be a power of two (TMEM allocation)");
   static_assert(kBNLocal * kElemBytes % 128 == 0, "B tile must be whole 128-byte boxes");
@@ -462,7 +466,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
   const bool is_leader = (cta_rank == 0);
   // K split over a cluster (see UmmaGemmParams::cluster_k): the fp32 split kernel and the int8
   // kernel, single CTAs only
-  constexpr bool kClusterKCapable = kCtaGroup == 1 && (kSplit || kKind == ptx::MmaKind::I8);
+  constexpr bool kClusterKCapable = kCtaGroup == 1 && (kSplit || ptx::is_8bit(kKind));
   const unsigned ksplit = (kClusterKCapable && p.cluster_k > 1) ? p.cluster_k : 1u;
   const unsigned krank = ksplit > 1 ? ptx::cluster_ctarank() : 0u;
   const bool in_cluster = (kCtaGroup == 2) || ksplit > 1;
@@ -745,6 +749,11 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
           const unsigned prow = ptm * Cfg::kTileM + cta_rank * Cfg::kBM + q * 32 + (lane & 3u) * 8;
           if (lane < 4 && prow < p.M)
             ptx::prefetch_l2(p.rsA + static_cast<size_t>(p.strideRsA) * pb + prow);
+        } else if constexpr (kKind == ptx::MmaKind::S8) {
+          if (pcol < p.N && lane * 8 < BN) {
+            ptx::prefetch_l2(p.b_scales + pcol);
+            if (p.bias) ptx::prefetch_l2(p.bias + pcol);
+          }
         } else {
           if (p.bias && pcol < p.N && lane * 8 < BN) ptx::prefetch_l2(p.bias + pcol);
         }
@@ -762,6 +771,8 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
               const unsigned col = wcol0 + i * 32 + lane;
               stage_one[i * 32 + lane] = col < p.N ? static_cast<uint32_t>(__ldg(rsb + col)) : 0u;
             }
+          } else if constexpr (kKind == ptx::MmaKind::S8) {
+            // (this kind reads its column terms from here for every tile, see the store loop)
           } else {
 #pragma unroll
             for (int i = 0; i < kWarpCols / 32; ++i) {
@@ -945,11 +956,95 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
           if (row_ok)
             row_term += static_cast<uint32_t>(__ldg(p.rsA + static_cast<size_t>(p.strideRsA) * b + row)) * ob;
         }
+        float row_scale = 0.f;
+        if constexpr (kKind == ptx::MmaKind::S8) row_scale = row_ok ? __ldg(p.a_scales + row) : 0.f;
         bounded_wait<false>(tmem_full(acc), acc_ph, TFCCB200_DEV_TIMEOUT_EPILOGUE, ctl);
         ptx::tc_fence_after_sync();
         const uint32_t taddr = lane_addr + acc * BN;
         const EpiTarget& tgt = *tgt_smem;
-        if constexpr (kKind != ptx::MmaKind::I8) {
+        if constexpr (kKind == ptx::MmaKind::S8) {
+          // fp32 results from the exact int32 sums: one column block of 32 after the other goes
+          // through the warp's staging block, which all four warps of the quarter keep for
+          // themselves, and leaves by TMA store (or, for rows that are no multiple of 16 bytes, by
+          // 128-byte row segments).
+          const int act = tgt.activation;
+          unsigned c_lo = 0, c_hi = BN / 32;
+          const uint4* red = nullptr;
+          unsigned qper = 0, ew = warp - Cfg::kFirstEpilogueWarp;
+          if (ksplit > 1) {
+            // as for I8: every rank receives the other ranks' sums of its own columns
+            const unsigned slice = BN / ksplit;
+            qper = slice / 4;
+            if (ew == 0 && lane == 0)
+              for (unsigned r = 0; r < ksplit; ++r)
+                if (r != krank) ptx::mbar_arrive_cluster(ptx::mapa(red_free, r));
+            bounded_wait<true>(red_free, 0u, TFCCB200_DEV_TIMEOUT_EPILOGUE, ctl);
+            for (unsigned d = 0; d < ksplit; ++d) {
+              if (d == krank) continue;
+              const unsigned si2 = krank < d ? krank : krank - 1;  // this rank among d's sources
+              const uint32_t remote = ptx::mapa(smem_base, d);
+              for (unsigned c = 0; c < slice / 32; ++c) {
+                uint32_t r[32];
+                ptx::tmem_ld_32x32(taddr + d * slice + c * 32, r);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                  ptx::st_shared_cluster_v4_b32(
+                      remote + 16u * (((si2 * Cfg::kNumEpilogueWarps + ew) * qper + c * 8 + v) * 32 + lane),
+                      r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+              }
+              ptx::mbar_arrive_cluster(ptx::mapa(red_ready, d));
+            }
+            bounded_wait<true>(red_ready, 0u, TFCCB200_DEV_TIMEOUT_EPILOGUE, ctl);
+            red = reinterpret_cast<const uint4*>(smem_gen);
+            c_lo = krank * (slice / 32);
+            c_hi = c_lo + slice / 32;
+          }
+#pragma unroll 1
+          for (unsigned c = c_lo; c < c_hi; ++c) {
+            const unsigned colb = col0 + c * 32;
+            if (colb >= pN) break;  // warp-uniform
+            // lane l keeps column l's scale and bias
+            const bool col_ok = colb + lane < pN;
+            const float my_scale = col_ok ? __ldg(p.b_scales + colb + lane) : 0.f;
+            const float my_bias = (pbias && col_ok) ? __ldg(pbias + colb + lane) : 0.f;
+            uint32_t r[32];
+            ptx::tmem_ld_32x32(taddr + c * 32, r);
+            ptx::tmem_ld_wait();
+            if (red) {
+              for (unsigned s2 = 0; s2 + 1 < ksplit; ++s2) {
+#pragma unroll
+                for (int v = 0; v < 8; ++v) {
+                  const uint4 t = red[((s2 * Cfg::kNumEpilogueWarps + ew) * qper + (c - c_lo) * 8 + v) * 32 + lane];
+                  r[4 * v] += t.x; r[4 * v + 1] += t.y; r[4 * v + 2] += t.z; r[4 * v + 3] += t.w;
+                }
+              }
+            }
+            if (tgt.tma_store) epi_tma_stage_free(lane);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float y = fmaf(static_cast<float>(static_cast<int>(r[j])) * row_scale,
+                                   __shfl_sync(0xffffffffu, my_scale, j), __shfl_sync(0xffffffffu, my_bias, j));
+              r[j] = __float_as_uint(act != TFCCB200_ACT_NONE ? apply_activation(y, act) : y);
+            }
+#pragma unroll
+            for (int qq = 0; qq < 8; ++qq)
+              epi_stage_chunk(stage, lane, qq, make_uint4(r[4 * qq], r[4 * qq + 1], r[4 * qq + 2], r[4 * qq + 3]));
+            if (tgt.tma_store) {
+              epi_tma_store_block(stage, lane, &tmapC, colb, row0, b);
+            } else {
+              __syncwarp();
+#pragma unroll 4
+              for (unsigned rr = 0; rr < 32; ++rr) {
+                const uint32_t v = stage[rr * 32 + (((lane >> 2) ^ (rr & 7u)) << 2) + (lane & 3u)];
+                if (row0 + rr < pM && col_ok)
+                  tgt.dst[0][static_cast<unsigned long long>(row0 + rr) * tgt.ldc + colb + lane] = v;
+              }
+              __syncwarp();
+            }
+          }
+          if (tgt.tma_store) epi_tma_stage_free(lane);
+        } else if constexpr (kKind != ptx::MmaKind::I8) {
           if (tgt.tma_store) {
             const int act = tgt.activation;
 #pragma unroll 1

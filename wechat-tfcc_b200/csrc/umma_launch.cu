@@ -43,12 +43,13 @@ EncodeFn encode_fn() {
 // ragged M, N and K tails free.
 bool make_tmap(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const void* base,
                uint64_t row_elems, uint64_t rows, uint64_t batch, uint64_t batch_stride_elems,
-               uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+               uint32_t box_rows, CUtensorMapSwizzle swizzle, uint64_t row_pitch_elems = 0) {
   EncodeFn fn = encode_fn();
   if (!fn) return false;
+  const uint64_t pitch = row_pitch_elems ? row_pitch_elems : row_elems;
   cuuint64_t dims[3] = {row_elems, rows, batch};
-  uint64_t bstride = batch_stride_elems ? batch_stride_elems : row_elems * rows;
-  cuuint64_t strides[2] = {row_elems * elem_bytes, bstride * elem_bytes};
+  uint64_t bstride = batch_stride_elems ? batch_stride_elems : pitch * rows;
+  cuuint64_t strides[2] = {pitch * elem_bytes, bstride * elem_bytes};
   cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / elem_bytes), box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
@@ -125,7 +126,7 @@ int launch(cudaStream_t stream, const CUtensorMap& ta, const CUtensorMap& tb, Um
   unsigned cluster = kCtaGroup;
   if (p.cluster_k > 1) {
     // K split over a cluster: one tile per cluster, all tiles resident at once
-    constexpr bool kCapable = kCtaGroup == 1 && (kSplit || kKind == ptx::MmaKind::I8);
+    constexpr bool kCapable = kCtaGroup == 1 && (kSplit || ptx::is_8bit(kKind));
     if (!kCapable || total * p.cluster_k > static_cast<unsigned>(sm_count))
       return TFCCB200_EUNSUPPORTED;
     // fp32: the other ranks' whole partial tiles meet in rank 0's stage buffers; int8: every
@@ -720,6 +721,46 @@ int umma_qgemm(const QgemmArgs& a, bool pair) {
     return launch<I, false, 1, 128, 6>(a.stream, ta, tb, p, sms);
   }
   return launch<I, false, 2, 256, 6>(a.stream, ta, tb, p, sms);
+}
+
+bool umma_s8_gemm_supported(const S8GemmArgs& a) {
+  // K and N may be anything: the tensor maps know them, and the pitches are what TMA wants to be
+  // multiples of 16 bytes.
+  return a.lda % 16 == 0 && a.ldb % 16 == 0 && aligned16(a.A) && aligned16(a.B);
+}
+
+int umma_s8_gemm(const S8GemmArgs& a, int force_pair) {
+  cudaError_t ce;
+  const DeviceInfo* di = current_device_info(&ce);
+  if (!di) return static_cast<int>(ce);
+  if (di->cc_major != 10) return TFCCB200_EUNSUPPORTED;
+  const I8Plan plan = plan_i8(a.M, a.N, a.K, 1, di->sm_count, force_pair);
+
+  CUtensorMap ta, tb;
+  if (!make_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.A, a.K, a.M, 1, 0, 128, CU_TENSOR_MAP_SWIZZLE_128B, a.lda) ||
+      !make_tmap(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.B, a.N, a.K, 1, 0, 128, CU_TENSOR_MAP_SWIZZLE_128B, a.ldb))
+    return TFCCB200_EINVAL;
+
+  UmmaGemmParams p = {};
+  p.num_dst = 1;
+  p.dst[0] = a.C;
+  p.ldc = a.N;
+  p.bias = a.bias;
+  p.activation = a.activation;
+  p.a_scales = a.a_scales;
+  p.b_scales = a.b_scales;
+  p.cluster_k = plan.pair ? 1 : plan.cluster_k;
+  p.M = a.M; p.N = a.N; p.K = a.K; p.batch = 1;
+  p.strideC = static_cast<unsigned long long>(a.M) * a.N;
+  p.status = a.status;
+  p.timeout_ns = kDefaultTimeoutNs;
+  p.flag_timeout_ns = kDefaultTimeoutNs;
+
+  constexpr auto S = ptx::MmaKind::S8;
+  const int sms = di->sm_count;
+  if (plan.pair) return launch<S, false, 2, 256, 6>(a.stream, ta, tb, p, sms);
+  if (plan.bn == 256) return launch<S, false, 1, 256, 4>(a.stream, ta, tb, p, sms);
+  return launch<S, false, 1, 128, 6>(a.stream, ta, tb, p, sms);
 }
 
 }  // namespace tfccb200

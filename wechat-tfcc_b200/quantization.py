@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 
 from . import exceptions
-from ._lib import PATHS, check, lib
+from ._lib import ACTIVATIONS, PATHS, check, lib
 from .session import get_session
 
 _REDUCE = {torch.uint8: "tfccb200_reduce_sum_u8", torch.int8: "tfccb200_reduce_sum_s8",
@@ -255,3 +255,121 @@ def matmul_host(a, b, min_a, max_a, min_b, max_b):
                                          k, batch)
     check(st)
     return out, mn.value, mx.value
+
+
+# ---- one scale per token and per channel --------------------------------------------------------
+
+
+def _rows(t, name, dtype):
+    """(pointer pitch in elements, rows, columns) of a rank >= 2 CUDA tensor whose last dimension is
+    contiguous and whose rows are evenly spaced."""
+    if not isinstance(t, torch.Tensor) or t.dim() < 2 or t.numel() == 0:
+        raise exceptions.InvalidArgumentError(f"invalid tensor {name}")
+    if t.dtype != dtype:
+        raise exceptions.NotImplementedError(f"{name}: implemented for {dtype}, got {t.dtype}")
+    if not t.is_cuda:
+        raise exceptions.InvalidArgumentError(f"{name} must be a CUDA tensor")
+    shape, stride = t.shape, t.stride()
+    cols = shape[-1]
+    rows, pitch = shape[-2], stride[-2]
+    for d in range(t.dim() - 3, -1, -1):
+        if shape[d] != 1:
+            if rows == 1:
+                pitch = stride[d]
+            elif stride[d] != rows * pitch:
+                raise exceptions.InvalidArgumentError(f"{name}: rows must be evenly spaced")
+            rows *= shape[d]
+    if rows == 1:
+        pitch = max(pitch, cols)  # the stride of a single row says nothing
+    if (cols != 1 and stride[-1] != 1) or pitch < cols:
+        raise exceptions.InvalidArgumentError(f"{name}: rows must be contiguous and must not overlap")
+    return pitch, rows, cols
+
+
+def _vector(t, name, size, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or \
+            t.numel() != size or not t.is_contiguous():
+        raise exceptions.InvalidArgumentError(f"invalid tensor {name}: expected {size} contiguous float32 on {device}")
+    return t.data_ptr()
+
+
+def quantize_tokens(a: torch.Tensor):
+    """``(codes, scales)`` of float32 rows ``[..., K]`` (rank >= 2): ``scales = max|row| / 127``
+    (float32, shape ``[...]``) and ``codes = round_half_even(row / scale)``, int8 in [-127, 127],
+    decided by the exact quotient.  A zero row has scale 0; a row with an infinity or a NaN has
+    scale NaN and codes 0.  The codes' rows start on 16-byte boundaries (a view of a wider
+    buffer when K is no multiple of 16), which is the layout :func:`matmul_scaled` is fast on."""
+    pitch, rows, cols = _rows(a, "a", torch.float32)
+    wide = (cols + 15) // 16 * 16
+    shape = list(a.shape)
+    codes = torch.empty(shape[:-1] + [wide], dtype=torch.int8, device=a.device)
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=a.device)
+    sess = get_session(a.device)
+    with torch.cuda.device(a.device):
+        check(lib.tfccb200_quantize_tokens_f32(sess.stream_ptr, a.data_ptr(), pitch, rows, cols,
+                                               codes.data_ptr(), wide, scales.data_ptr()))
+    return codes[..., :cols], scales
+
+
+def quantize_channels(w: torch.Tensor):
+    """``(codes, scales)`` of a float32 weight ``[K, N]`` with one scale per output channel (column),
+    by the rule of :func:`quantize_tokens`: a one-time preparation when a weight is loaded.  The
+    codes come back as ``[K, N]`` with rows that start on 16-byte boundaries."""
+    if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.numel() == 0:
+        raise exceptions.InvalidArgumentError("invalid tensor w")
+    codes, scales = quantize_tokens(w.t().contiguous())
+    k, n = w.shape
+    out = torch.zeros(k, (n + 15) // 16 * 16, dtype=torch.int8, device=w.device)
+    out[:, :n] = codes.t()
+    return out[:, :n], scales
+
+
+def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+                  bias: torch.Tensor | None = None, *, activation: str | None = None,
+                  path: str = "auto") -> torch.Tensor:
+    """``act(a_scales[..., m] * b_scales[n] * (a . b)[..., m, n] + bias[n])`` in float32, the int32
+    products of the int8 codes ``a`` ``[..., M, K]`` and ``b`` ``[K, N]`` summed exactly.
+    ``activation="gelu"`` applies the erf GELU.  Operands whose rows start on 16-byte boundaries
+    (as the quantize functions here return them) run on the tensor cores."""
+    lda, m, k = _rows(a, "a", torch.int8)
+    ldb, kb, n = _rows(b, "b", torch.int8)
+    if b.dim() != 2 or kb != k:
+        raise exceptions.InvalidArgumentError("tensor a and b don't match")
+    if b.device != a.device:
+        raise exceptions.InvalidArgumentError("operands live on different devices")
+    if activation not in ACTIVATIONS or path not in PATHS:
+        raise exceptions.InvalidArgumentError("unknown activation or path")
+    sa = _vector(a_scales, "a_scales", m, a.device)
+    sb = _vector(b_scales, "b_scales", n, a.device)
+    sbias = None if bias is None else _vector(bias, "bias", n, a.device)
+    out = torch.empty(list(a.shape[:-1]) + [n], dtype=torch.float32, device=a.device)
+    sess = get_session(a.device)
+    with torch.cuda.device(a.device):
+        check(lib.tfccb200_qgemm_scaled_s8(sess.stream_ptr, a.data_ptr(), lda, sa, b.data_ptr(), ldb,
+                                           sb, sbias, out.data_ptr(), m, n, k,
+                                           ACTIVATIONS[activation], PATHS[path], sess.status_ptr))
+    return out
+
+
+def linear(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None,
+           *, activation: str | None = None) -> torch.Tensor:
+    """``matmul_scaled(*quantize_tokens(x), b, b_scales, bias)`` in one call: float32 ``x``
+    ``[..., K]`` in, float32 ``[..., N]`` out, the codes of ``x`` in the session's workspace."""
+    ldx, m, k = _rows(x, "x", torch.float32)
+    ldb, kb, n = _rows(b, "b", torch.int8)
+    if b.dim() != 2 or kb != k:
+        raise exceptions.InvalidArgumentError("tensor x and b don't match")
+    if b.device != x.device:
+        raise exceptions.InvalidArgumentError("operands live on different devices")
+    if activation not in ACTIVATIONS:
+        raise exceptions.InvalidArgumentError("unknown activation")
+    sb = _vector(b_scales, "b_scales", n, x.device)
+    sbias = None if bias is None else _vector(bias, "bias", n, x.device)
+    out = torch.empty(list(x.shape[:-1]) + [n], dtype=torch.float32, device=x.device)
+    sess = get_session(x.device)
+    with torch.cuda.device(x.device):
+        ws_ptr, ws_len = sess.workspace(lib.tfccb200_qlinear_workspace(m, k))
+        check(lib.tfccb200_qlinear_f32(sess.stream_ptr, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias,
+                                       out.data_ptr(), m, n, k, ACTIVATIONS[activation], ws_ptr, ws_len,
+                                       sess.status_ptr))
+    return out

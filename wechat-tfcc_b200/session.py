@@ -56,6 +56,9 @@ class Session:
         st = int(self._status.item())
         if st:
             self._status.zero_()
+            if not st & 0xF:  # no wait ran out
+                raise exceptions.InvalidArgumentError(
+                    f"a cache operator met sequences or pages out of range (bits 0x{st:x})")
             raise exceptions.RuntimeError(-6, f"a kernel abandoned a bounded wait (bits 0x{st:x})")
 
 
