@@ -1,0 +1,203 @@
+// How the attention kernels share out their work.
+//
+// An item is a tile of kRows query rows of one kv head of one sequence (row r of a sequence's head
+// is new token r / group, query head r % group of the head's group), and its units are the blocks
+// of kBlockKeys cached tokens that the tile's last row sees.  Lengths are device data and differ, so no
+// grid the host could choose would be even: instead the units of all items are laid end to
+// end (sequence, head, tile, block) and every CTA takes an equal range of them.  A range may begin
+// and end inside an item.  Items that lie whole in one range are finished there; the pieces of a
+// cut one go to scratch as unnormalised sums with their maximum, and the merge kernel adds
+// them in key order.  Cuts depend on lengths and grid alone, so results repeat bit by bit.
+#pragma once
+
+#include "cache.cuh"
+
+namespace tfccb200 {
+
+constexpr unsigned kBlockKeys = 128;
+// Sequences with up to this many rows per kv head go to the few-rows kernel.
+constexpr unsigned kFewRows = 16;
+
+struct CacheAttention {
+  CacheParams c;
+  const float* q;
+  float* out;
+  unsigned long long ldq, ldo;
+  unsigned heads, group;  // group = heads / kv_heads
+  unsigned min_rows, max_rows;  // rows per kv head of the sequences this launch takes
+  unsigned grid;          // CTAs that share the units
+  int causal;
+  float scale;            // times log2(e)
+  float* scratch;         // pieces, see piece_*; nullptr when no item can be cut
+};
+
+// Blocks of one tile; one at least, so that a row that sees nothing is still written.
+template <int kRows>
+__device__ __forceinline__ unsigned tile_blocks(const CacheAttention& a, const DeviceSequence& s, unsigned tile) {
+  int end = s.length;
+  if (a.causal) {
+    const unsigned last = min(static_cast<unsigned>(s.count) * a.group, (tile + 1) * kRows) - 1;
+    end = s.length - s.count + static_cast<int>(last / a.group) + 1;
+  }
+  return end <= 0 ? 1u : (static_cast<unsigned>(end) + kBlockKeys - 1) / kBlockKeys;
+}
+
+template <int kRows>
+__device__ __forceinline__ unsigned sequence_tiles(const CacheAttention& a, const DeviceSequence& s) {
+  const unsigned long long rows = static_cast<unsigned long long>(s.count) * a.group;
+  if (rows == 0 || rows < a.min_rows || rows > a.max_rows) return 0;
+  return static_cast<unsigned>((rows + kRows - 1) / kRows);
+}
+
+// Units of one kv head of a sequence.
+template <int kRows>
+__device__ __forceinline__ unsigned head_units(const CacheAttention& a, const DeviceSequence& s) {
+  const unsigned tiles = sequence_tiles<kRows>(a, s);
+  unsigned n = 0;
+  for (unsigned t = 0; t < tiles; ++t) n += tile_blocks<kRows>(a, s, t);
+  return n;
+}
+
+struct ScheduleShared {
+  unsigned long long sums[33];
+  unsigned long long rem;
+  int seq;
+};
+
+// Sum of v over the block (to every thread).
+template <int kThreads>
+__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, ScheduleShared* sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31u) == 0) sh->sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  unsigned long long t = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) t += sh->sums[w];
+  return t;
+}
+
+// Units of all sequences.  `mine` keeps those of sequence threadIdx.x for find_unit.
+template <int kRows, int kThreads>
+__device__ __forceinline__ unsigned long long all_units(const CacheAttention& a, ScheduleShared* sh,
+                                                        unsigned long long* mine) {
+  unsigned long long n = 0;
+  *mine = 0;
+  for (unsigned b = threadIdx.x; b < a.c.batch; b += kThreads) {
+    const unsigned long long u =
+        static_cast<unsigned long long>(head_units<kRows>(a, load_sequence(a.c, b))) * a.c.kv_heads;
+    if (b < kThreads) *mine = u;
+    n += u;
+  }
+  return block_sum<kThreads>(n, sh);
+}
+
+// The sequence that unit u (< all units) belongs to -> sh->seq, and u's place within it -> sh->rem.
+template <int kRows, int kThreads>
+__device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long long u, unsigned long long mine,
+                                          ScheduleShared* sh) {
+  unsigned long long before = 0;  // units of the sequences of earlier rounds
+  for (unsigned b0 = 0; b0 < a.c.batch; b0 += kThreads) {
+    const unsigned b = b0 + threadIdx.x;
+    if (b0) mine = b < a.c.batch
+                       ? static_cast<unsigned long long>(head_units<kRows>(a, load_sequence(a.c, b))) * a.c.kv_heads
+                       : 0ull;
+    unsigned long long v = mine;  // inclusive scan over the block
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long t = __shfl_up_sync(0xffffffffu, v, o);
+      if ((threadIdx.x & 31u) >= static_cast<unsigned>(o)) v += t;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31u) == 31u) sh->sums[threadIdx.x >> 5] = v;
+    __syncthreads();
+    unsigned long long total = 0;
+    unsigned long long base = before;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < static_cast<int>(threadIdx.x >> 5)) base += sh->sums[w];
+      total += sh->sums[w];
+    }
+    if (mine && base + v - mine <= u && u < base + v) {
+      sh->seq = static_cast<int>(b);
+      sh->rem = u - (base + v - mine);
+    }
+    before += total;
+    if (before > u) break;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ unsigned long long range_begin(unsigned long long units, unsigned grid, unsigned cta) {
+  return units / grid * cta + units % grid * cta / grid;
+}
+
+// Walks the items of a range of units.
+template <int kRows>
+struct ItemWalk {
+  const CacheAttention& a;
+  unsigned long long left;  // units still to come, this item's included
+  unsigned long long rem;   // this item's first unit within the sequence
+  int b;
+  DeviceSequence seq;
+  unsigned per_head, head, tile, blocks;  // `blocks`: all of the item's
+  unsigned lo, hi;                        // this range's blocks of it
+
+  __device__ ItemWalk(const CacheAttention& a_, unsigned long long units, const ScheduleShared* sh)
+      : a(a_), left(units), rem(0), b(0), per_head(0), head(0), tile(0), blocks(0), lo(0), hi(0) {
+    if (left == 0) return;
+    b = sh->seq;
+    rem = sh->rem;
+    seq = load_sequence(a.c, b);
+    per_head = head_units<kRows>(a, seq);
+    place();
+  }
+  __device__ void place() {
+    head = static_cast<unsigned>(rem / per_head);
+    unsigned at = static_cast<unsigned>(rem % per_head);
+    tile = 0;
+    while (true) {
+      blocks = tile_blocks<kRows>(a, seq, tile);
+      if (at < blocks) break;
+      at -= blocks;
+      ++tile;
+    }
+    lo = at;
+    hi = static_cast<unsigned>(min(static_cast<unsigned long long>(blocks), at + left));
+  }
+  __device__ bool done() const { return left == 0; }
+  __device__ bool whole() const { return lo == 0 && hi == blocks; }
+  __device__ void next() {
+    const unsigned n = hi - lo;
+    left -= n;
+    rem += n;
+    if (left == 0) return;
+    while (rem >= static_cast<unsigned long long>(per_head) * a.c.kv_heads) {
+      rem = 0;
+      do {
+        ++b;
+        seq = load_sequence(a.c, b);
+        per_head = head_units<kRows>(a, seq);
+      } while (per_head == 0);  // units are left, so a sequence that has some follows
+    }
+    place();
+  }
+};
+
+// The pieces of cut items: a CTA has at most one that begins inside an item (slot 0) and one that
+// begins with it (slot 1).  A piece: kRows maxima (log2 units), kRows weight sums, kRows * DIM sums.
+template <int kRows, int DIM>
+__host__ __device__ constexpr size_t piece_floats() { return static_cast<size_t>(kRows) * (DIM + 2); }
+template <int kRows, int DIM>
+__device__ __forceinline__ float* piece(const CacheAttention& a, unsigned cta, bool begins) {
+  return a.scratch + (2ull * cta + (begins ? 1u : 0u)) * piece_floats<kRows, DIM>();
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace tfccb200
