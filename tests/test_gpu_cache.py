@@ -9,7 +9,13 @@ tolerance is derived per output element.  With A = sum_j p_j |v_j| (p the exact 
   * weights times value scales as two 11-bit terms, exp2 and the scalings: 2^-20 A; the product's 16
     accumulation steps of a block 2^-19 A;
   * the running sums over blocks and the sum of the weights, in fp32: (256 + n / 64) 2^-24 A for n
-    keys (a thread adds at most 128 weights of a block one after another, and blocks one by one)."""
+    keys (a thread adds at most 128 weights of a block one after another, and blocks one by one);
+  * fp16 ends: a weight is held in units that put the largest value scale of its block, rounded up to
+    a power of two E <= 2 max vs, times the largest p at 2^10 or more, and the low term's spacing never
+    falls below 2^-24, so a weight has an absolute error of at most 2^-25 2^-10 E however small it
+    is.  With |vc| <= 127 and a sum of weights of at least 1 that is 2^-35 * 2 max vs * 127 per
+    key, n times: the only term that does not shrink with A (it shows where one key takes nearly all the
+    weight and its value is exactly 0)."""
 import math
 
 import numpy as np
@@ -93,7 +99,10 @@ def expected(s, q, heads, scale, causal):
             out[row:row + new] = torch.einsum("hgij,jhd->ihgd", p, v).reshape(new, heads, s.dim)
             a = torch.einsum("hgij,jhd->ihgd", p, v.abs())
             ds = size.amax(-1).permute(2, 0, 1)[..., None] * C_SCORE
-            tol[row:row + new] = (a * (2 * ds + 2.0 ** -20 + 2.0 ** -19 + (256 + n / 64) * 2.0 ** -24)).reshape(new, heads, s.dim)
+            page, slot = s.where(b)
+            top = s.cache.value_scales[page, :, slot].double().amax()
+            end = n * 2.0 ** -34 * 127 * top
+            tol[row:row + new] = (a * (2 * ds + 2.0 ** -20 + 2.0 ** -19 + (256 + n / 64) * 2.0 ** -24) + end).reshape(new, heads, s.dim)
         row += new
     return out.view(s.rows, -1), tol.view(s.rows, -1)
 
@@ -356,7 +365,7 @@ def test_pool_beyond_four_gigabytes(pkg):
         st = torch.tensor([0, new], dtype=torch.int32, device=dev())
         got = pkg.cache.attention(cache, q, st, lens, table)
         s = Setup.__new__(Setup)
-        s.rows, s.news, s.lengths, s.kv, s.dim = new, [new], [n], kv, dim
+        s.rows, s.news, s.lengths, s.kv, s.dim, s.page, s.cache, s.table = new, [new], [n], kv, dim, page, cache, table
         s.held = lambda b: (rk.double().view(n, kv, dim), rv.double().view(n, kv, dim))
         want, tol = expected(s, q, 16, 1 / math.sqrt(dim), True)
         compare(got, want, tol * 2, new)  # (the values read back carry one more rounding, 2^-24)

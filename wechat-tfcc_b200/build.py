@@ -24,7 +24,8 @@ LIB = HERE / "libtfcc_b200.so"
 OBJ_DIR = HERE / "build"
 SOURCES = ["capi.cu", "umma_launch.cu", "simt_kernels.cu", "quantize_kernels.cu",
            "nn_kernels.cu", "group.cu", "attention.cu", "cluster_simt.cu",
-           "s8_kernels.cu", "cache.cu", "cache_attention.cu"]
+           "s8_kernels.cu", "cache.cu", "cache_attention.cu",
+           "cache_attention_many.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

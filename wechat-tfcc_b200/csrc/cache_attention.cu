@@ -1,5 +1,5 @@
-// Attention of new tokens over the paged 8-bit cache: the kernel for few rows, the one that joins
-// the pieces of shared items, and the choice between the kernels.
+// Attention of new tokens over the paged 8-bit cache: the kernel for few rows, and the choice
+// between it and the one for many (cache_attention_many.cu).
 //
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j,   k_j = ks_j kc_j, v_j = vs_j vc_j (s8 codes)
 //
@@ -14,9 +14,9 @@
 // the one-pass form: running maximum and sum in fp32, sums rescaled when the maximum grows.
 #include <cuda_runtime.h>
 
-#include <atomic>
+#include <algorithm>
 
-#include "cache_schedule.cuh"
+#include "cache_attention.cuh"
 #include "internal.h"
 #include "pdl.cuh"
 #include "ptx.cuh"
@@ -68,36 +68,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint4 a, uint32_t b0, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-
-// Two floats as packed fp16 (first in the low half), and what the rounding left over.
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
-}
-__device__ __forceinline__ float half_low(uint32_t h) {
-  float f;
-  asm("{.reg .f16 l, u; mov.b32 {l, u}, %1; cvt.f32.f16 %0, l;}" : "=f"(f) : "r"(h));
-  return f;
-}
-__device__ __forceinline__ float half_high(uint32_t h) {
-  float f;
-  asm("{.reg .f16 l, u; mov.b32 {l, u}, %1; cvt.f32.f16 %0, u;}" : "=f"(f) : "r"(h));
-  return f;
-}
-__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
-  return pack_half2(a - half_low(hi), b - half_high(hi));
-}
-
-// Codes (biased to unsigned by an exclusive or with 0x80) to fp16: the byte becomes the low mantissa
-// bits of 1024 + u, from which 1152 is taken.
-__device__ __forceinline__ uint32_t unbias(uint32_t h) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
-  return r;
-}
-__device__ __forceinline__ uint32_t codes_low(uint32_t u) { return unbias(__byte_perm(u, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t codes_high(uint32_t u) { return unbias(__byte_perm(u, 0x64646464u, 0x4342)); }
 
 // Where 16-byte chunk `c` of code row `r` of a stage lies.  K rows are read by four lanes per row,
 // V rows by lanes that share a chunk over four rows of one parity; both orders then touch eight different
@@ -459,130 +429,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
   }
 }
 
-// ---- the pieces of cut items ---------------------------------------------------------------------
-//
-// CTA c looks at the boundary between ranges c and c + 1 (those of the attention kernel).  If that is the
-// first boundary inside an item, it adds the item's pieces in key order; blockIdx.y shares out
-// the item's elements.
-template <int DIM, int ROWS>
-__global__ void __launch_bounds__(256) cache_attention_merge_kernel(const __grid_constant__ CacheAttention a) {
-  __shared__ ScheduleShared sched;
-  pdl_release();
-  pdl_wait();
-  unsigned long long mine;
-  const unsigned long long units = all_units<ROWS, 256>(a, &sched, &mine);
-  const unsigned c = blockIdx.x + 1;
-  const unsigned long long at = range_begin(units, a.grid, c);
-  if (at >= units) return;
-  find_unit<ROWS, 256>(a, at, mine, &sched);
-  const ItemWalk<ROWS> item(a, 1, &sched);
-  if (item.lo == 0) return;  // the boundary lies between two items
-  const unsigned long long begin = at - item.lo, end = begin + item.blocks;
-  if (range_begin(units, a.grid, c - 1) > begin) return;  // not the item's first
-  const unsigned rows = static_cast<unsigned>(item.seq.count) * a.group;
-  for (unsigned e = (blockIdx.y * 256 + threadIdx.x) * 4; e < ROWS * DIM; e += gridDim.y * 1024) {
-    const unsigned r = e / DIM, d = e % DIM, row = item.tile * ROWS + r;
-    if (row >= rows) continue;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    unsigned long long from = begin;
-    for (unsigned k = c - 1; from < end; ++k) {
-      const unsigned long long to = range_begin(units, a.grid, k + 1);
-      if (to <= from) continue;  // an empty range, or the part of range c - 1 before the item
-      const float* p = piece<ROWS, DIM>(a, k, k == c - 1);
-      const float pm = __ldg(p + r), pl = __ldg(p + ROWS + r);
-      const float4 y = __ldg(reinterpret_cast<const float4*>(p + 2 * ROWS + e));
-      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
-      const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
-      m = next;
-      l = f * l + g * pl;
-      acc.x = f * acc.x + g * y.x; acc.y = f * acc.y + g * y.y;
-      acc.z = f * acc.z + g * y.z; acc.w = f * acc.w + g * y.w;
-      from = to;
-    }
-    const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-    const unsigned tok = row / a.group;
-    float* dst = a.out + a.ldo * (static_cast<size_t>(item.seq.first) + tok) +
-                 (static_cast<size_t>(item.head) * a.group + row % a.group) * DIM + d;
-    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-  }
-}
-
-// ---- CUDA-core form for many rows (to be replaced) -----------------------------------------------
-template <int DIM>
-__global__ void __launch_bounds__(128) cache_attention_simple_kernel(const CacheAttention a) {
-  constexpr int kPer = DIM / 32;
-  __shared__ float sh_m[4], sh_l[4], sh_o[4][DIM];
-  pdl_release();
-  pdl_wait();
-  check_all_sequences(a.c);
-  const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const unsigned row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
-  const int b = sequence_of_row(a.c, row);
-  if (b < 0) return;
-  const DeviceSequence seq = load_sequence(a.c, b);
-  if (!seq.ok || seq.count * a.group < a.min_rows) return;
-  int sees = seq.length;
-  if (a.causal) sees = seq.length - seq.count + (static_cast<int>(row) - seq.first) + 1;
-  const float* q = a.q + a.ldq * row + head * DIM + lane * kPer;
-  float qr[kPer], o[kPer], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) qr[i] = q[i] * a.scale, o[i] = 0.f;
-  for (int j = warp; j < sees; j += 4) {
-    const int page = page_of(a.c, b, j);
-    float s = 0.f, vs = __uint_as_float(0x7fffffffu), v[kPer];
-    if (page >= 0) {
-      const size_t at = cache_slot(a.c, page, head / a.group, j);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) s += qr[i] * static_cast<float>(a.c.keys[at * DIM + lane * kPer + i]);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] = static_cast<float>(a.c.values[at * DIM + lane * kPer + i]);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= a.c.key_scales[at];
-      vs = a.c.value_scales[at];
-    } else {
-      s = vs;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] = 0.f;
-    }
-    const float m2 = fmaxf(m, s), al = m == -INFINITY ? 0.f : exp2f(m - m2), pr = exp2f(s - m2);
-    l = l * al + pr;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * al + pr * vs * v[i];
-    m = m2;
-  }
-  if (lane == 0) sh_m[warp] = m, sh_l[warp] = l;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) sh_o[warp][lane * kPer + i] = o[i];
-  __syncthreads();
-  if (threadIdx.x < DIM) {
-    const float top = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-    float sum = 0.f, acc = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      const float f = sh_l[w] == 0.f ? 0.f : exp2f(sh_m[w] - top);
-      sum += f * sh_l[w];
-      acc += f * sh_o[w][threadIdx.x];
-    }
-    a.out[a.ldo * row + head * DIM + threadIdx.x] = sees <= 0 ? 0.f : acc / sum;
-  }
-}
-
 // ---- host ----------------------------------------------------------------------------------------
-
-template <class K>
-int opt_in_smem(K kernel, int bytes, std::atomic<unsigned long long>& configured) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (!(configured.load(std::memory_order_acquire) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    configured.fetch_or(bit, std::memory_order_release);
-  }
-  return TFCCB200_OK;
-}
 
 constexpr unsigned kFewCtasPerSm = 2;
 
@@ -626,8 +473,12 @@ size_t cache_attention_workspace(const CacheAttentionArgs& a) {
   cudaError_t ce;
   const DeviceInfo* di = current_device_info(&ce);
   const size_t sms = di ? di->sm_count : 148;
-  if (a.max_length <= kBlockKeys) return 0;
-  return 2 * kFewCtasPerSm * sms * few_rows_of(a) * (a.cache.dim + 2) * sizeof(float);
+  if (a.max_length <= kBlockKeys) return 0;  // one block per item: nothing is cut
+  const size_t row = (a.cache.dim + 2) * sizeof(float);
+  const size_t few = 2 * kFewCtasPerSm * sms * few_rows_of(a) * row;
+  const bool many = static_cast<unsigned long long>(a.max_new) * (a.heads / a.cache.kv_heads) > kFewRows;
+  // the two kernels run one after the other and share it
+  return many ? std::max(few, 2 * sms * kManyRows * row) : few;
 }
 
 int cache_attention(const CacheAttentionArgs& args) {
@@ -658,11 +509,7 @@ int cache_attention(const CacheAttentionArgs& args) {
   if (static_cast<unsigned long long>(args.max_new) * a.group > kFewRows) {
     a.min_rows = kFewRows + 1;
     a.max_rows = 0xffffffffu;
-    const dim3 grid(args.cache.rows * args.heads);
-    cudaError_t e = wide ? launch_after_previous(cache_attention_simple_kernel<128>, grid, dim3(128), 0, args.cache.stream, a)
-                         : launch_after_previous(cache_attention_simple_kernel<64>, grid, dim3(128), 0, args.cache.stream, a);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    count_launch();
+    st = cache_attention_many(args, a, di->sm_count);
   }
   return st;
 }

@@ -1,0 +1,110 @@
+// What the two attention kernels over the paged 8-bit cache share beside the schedule: fp16 terms of fp32
+// values, codes as fp16, and the kernel that joins the pieces of cut items.
+#pragma once
+
+#include <atomic>
+
+#include "cache_schedule.cuh"
+#include "pdl.cuh"
+
+namespace tfccb200 {
+
+constexpr int kManyRows = 256;  // rows of an item of the many-rows kernel
+
+// Two floats as packed fp16 (first in the low half), and what the rounding left over.
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ float half_low(uint32_t h) {
+  float f;
+  asm("{.reg .f16 l, u; mov.b32 {l, u}, %1; cvt.f32.f16 %0, l;}" : "=f"(f) : "r"(h));
+  return f;
+}
+__device__ __forceinline__ float half_high(uint32_t h) {
+  float f;
+  asm("{.reg .f16 l, u; mov.b32 {l, u}, %1; cvt.f32.f16 %0, u;}" : "=f"(f) : "r"(h));
+  return f;
+}
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
+  return pack_half2(a - half_low(hi), b - half_high(hi));
+}
+
+// Codes (biased to unsigned by an exclusive or with 0x80) to fp16: the byte becomes the low mantissa
+// bits of 1024 + u, from which 1152 is taken.
+__device__ __forceinline__ uint32_t unbias(uint32_t h) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_low(uint32_t u) { return unbias(__byte_perm(u, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t codes_high(uint32_t u) { return unbias(__byte_perm(u, 0x64646464u, 0x4342)); }
+
+// ---- the pieces of cut items ---------------------------------------------------------------------
+//
+// CTA c looks at the boundary between ranges c and c + 1 (those of the attention kernel).  If that is the
+// first boundary inside an item, it adds the item's pieces in key order; blockIdx.y shares out
+// the item's elements.
+template <int DIM, int ROWS>
+static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const __grid_constant__ CacheAttention a) {
+  __shared__ ScheduleShared sched;
+  pdl_release();
+  pdl_wait();
+  unsigned long long mine;
+  const unsigned long long units = all_units<ROWS, 256>(a, &sched, &mine);
+  const unsigned c = blockIdx.x + 1;
+  const unsigned long long at = range_begin(units, a.grid, c);
+  if (at >= units) return;
+  find_unit<ROWS, 256>(a, at, mine, &sched);
+  const ItemWalk<ROWS> item(a, 1, &sched);
+  if (item.lo == 0) return;  // the boundary lies between two items
+  const unsigned long long begin = at - item.lo, end = begin + item.blocks;
+  if (range_begin(units, a.grid, c - 1) > begin) return;  // not the item's first
+  const unsigned rows = static_cast<unsigned>(item.seq.count) * a.group;
+  for (unsigned e = (blockIdx.y * 256 + threadIdx.x) * 4; e < ROWS * DIM; e += gridDim.y * 1024) {
+    const unsigned r = e / DIM, d = e % DIM, row = item.tile * ROWS + r;
+    if (row >= rows) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    unsigned long long from = begin;
+    for (unsigned k = c - 1; from < end; ++k) {
+      const unsigned long long to = range_begin(units, a.grid, k + 1);
+      if (to <= from) continue;  // an empty range, or the part of range c - 1 before the item
+      const float* p = piece<ROWS, DIM>(a, k, k == c - 1);
+      const float pm = __ldg(p + r), pl = __ldg(p + ROWS + r);
+      const float4 y = __ldg(reinterpret_cast<const float4*>(p + 2 * ROWS + e));
+      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
+      const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
+      m = next;
+      l = f * l + g * pl;
+      acc.x = f * acc.x + g * y.x; acc.y = f * acc.y + g * y.y;
+      acc.z = f * acc.z + g * y.z; acc.w = f * acc.w + g * y.w;
+      from = to;
+    }
+    const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+    const unsigned tok = row / a.group;
+    float* dst = a.out + a.ldo * (static_cast<size_t>(item.seq.first) + tok) +
+                 (static_cast<size_t>(item.head) * a.group + row % a.group) * DIM + d;
+    *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  }
+}
+
+template <class K>
+inline int opt_in_smem(K kernel, int bytes, std::atomic<unsigned long long>& configured) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured.fetch_or(bit, std::memory_order_release);
+  }
+  return TFCCB200_OK;
+}
+
+// Sequences with more than kFewRows rows per kv head (cache_attention_many.cu).
+int cache_attention_many(const CacheAttentionArgs& args, CacheAttention a, int sm_count);
+
+}  // namespace tfccb200
