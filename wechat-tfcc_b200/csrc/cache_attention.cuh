@@ -9,7 +9,7 @@
 
 namespace tfccb200 {
 
-constexpr int kManyRows = 256;  // rows of an item of the many-rows kernel
+constexpr int kManyRows = 128;  // rows of an item of the many-rows kernel
 
 // Two floats as packed fp16 (first in the low half), and what the rounding left over.
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -27,8 +27,36 @@ __device__ __forceinline__ float half_high(uint32_t h) {
   asm("{.reg .f16 l, u; mov.b32 {l, u}, %1; cvt.f32.f16 %0, u;}" : "=f"(f) : "r"(h));
   return f;
 }
+// Pairs of floats in the packed fp32 instructions of this architecture (one issue slot for two).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
-  return pack_half2(a - half_low(hi), b - half_high(hi));
+  const float2 r = unpair(fma2(pair(half_low(hi), half_high(hi)), pair(-1.f, -1.f), pair(a, b)));
+  return pack_half2(r.x, r.y);
 }
 
 // Codes (biased to unsigned by an exclusive or with 0x80) to fp16: the byte becomes the low mantissa

@@ -1,29 +1,38 @@
 // Attention over the paged 8-bit cache for many rows per kv head: chunks of prompts, tcgen05.
 //
-// An item is 256 query rows of one kv head (two halves of 128, the rows of one MMA) against a run
-// of 128-key blocks.  Arithmetic as in cache_attention.cu: K, V exact in fp16, Q and the weights as two
-// fp16 terms each, so per block and half
-//   S = Q_hi K^T + Q_lo K^T          A and B from shared memory, 128 x 128 fp32 in tensor memory
-//   P = exp2(S ks - m) vs            by one thread per row; hi and lo terms go back over S
+// An item is 128 query rows of one kv head (the rows of one MMA) against a run of 128-key blocks.
+// Arithmetic as in cache_attention.cu: K, V exact in fp16, Q and the weights as two fp16 terms each, so
+// per block
+//   S = Q_hi K^T + Q_lo K^T          A from tensor memory, K from shared memory, fp32 sums
+//   P = exp2(S ks - m) vs            hi and lo terms go back over S
 //   O_block = P_hi V + P_lo V        A from tensor memory, V as it lies (MN-major)
 //   O = O alpha + O_block            fp32 registers
 // The tensor core's accumulator narrows without rounding to nearest, which would bias O over
-// thousands of keys; summed from zero per block and added to registers it does not, and a block's own power
-// of two for the value scales comes along for nothing.
+// thousands of keys; summed from zero per block and added to registers it does not, and a block's
+// own power of two for the value scales comes along for nothing.
+//
+// Tensor memory (512 columns): Q_hi, Q_lo | S of even blocks | S of odd blocks | O_block.  With two S
+// buffers the tensor core computes the next block's scores while the weights of this one are made.
 //
 // Roles (512 threads, registers shifted with setmaxnreg):
-//   warp 0      issues the MMAs: PV of one half, then S of its next block, so that the other half's
-//               softmax runs while the tensor core is busy
+//   warp 0      issues the MMAs: S of block j + 1, then the products with V of block j
 //   warp 1      loads the blocks' scales
 //   warp 2      walks the schedule and hands the items to the others
 //   warps 4-7   turn codes into fp16 operand tiles (global -> registers -> shared memory): the tiles
 //               of K and V share a ring, one row's 64 values per 128-byte swizzled line
-//   warps 8-11  softmax, sums and output of half 0; warps 12-15 of half 1
-// Bound by the tensor core: 8 dim flops per (row, key) pair instead of the 4 counted, and its
-// operand reads from shared memory; the softmax's instructions come next.
+//   warps 8-15  softmax, sums and output of 16 rows each.  Tensor memory is read and written in the
+//               layout of matrix fragments, two rows and every fourth pair of keys per thread: 64 scores
+//               and 64 sums fit the registers, a row's maximum and sum are two shuffles, and a
+//               thread reads the scales of 32 keys instead of 128.  (A thread per row with all of
+//               its 128 sums left no registers to overlap the exponentials with and read every scale:
+//               3.4 times slower.)
+// Bound by the tensor core (8 dim flops per row and key instead of the 4 counted) and, close behind,
+// by the issue slots of the softmax.
 //
 // Every wait is bounded: on expiry a status bit is raised and all roles run to their end.
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "cache_attention.cuh"
 #include "internal.h"
@@ -36,7 +45,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kTileBytes = 128 * 128;  // 128 rows x 64 fp16, 128-byte swizzle
-constexpr int kRegsControl = 56, kRegsConvert = 88, kRegsSoftmax = 184;
+constexpr int kRegsControl = 48, kRegsConvert = 96, kRegsSoftmax = 184;
 static_assert(kRegsControl + kRegsConvert + 2 * kRegsSoftmax == 512, "shares of 128 registers per thread at launch");
 
 constexpr float kWeightTop = 1024.f;  // weights reach at most 2^10 times 2^kLazy, inside fp16's range
@@ -53,16 +62,16 @@ struct Item {  // what the roles need to know of an item; hi == 0 ends the walk
 template <int DIM>
 struct ManyLayout {
   static constexpr int kHalves = DIM / 64;               // 64-wide tiles of a row
-  static constexpr int kOperand = kHalves * kTileBytes;  // 128 rows of Q_hi, Q_lo, K or V
-  static constexpr int kRing = DIM == 128 ? 3 : 6;
-  static constexpr int kQ = 0;                           // [half][hi, lo]
-  static constexpr int kKv = 4 * kOperand;
-  static constexpr int kScales = kKv + kRing * kOperand;  // 2 x {ks[128], vr[128]}
+  static constexpr int kOperand = kHalves * kTileBytes;  // 128 rows of K or V
+  static constexpr int kRing = DIM == 128 ? 6 : 8;
+  static constexpr int kScales = kRing * kOperand;       // 2 x {ks[128], vr[128]}
   static constexpr int kItems = kScales + 2 * 1024;
   static constexpr int kBars = kItems + 2 * static_cast<int>(sizeof(Item));
-  static constexpr int kMisc = kBars + 8 * 32;            // tensor memory address, abort flag, value factors
+  static constexpr int kNumBars = 30;
+  static constexpr int kMisc = kBars + 8 * kNumBars;           // tensor memory address, abort flag, value factors
   static constexpr int kSched = kMisc + 16;
   static constexpr int kSmem = kSched + static_cast<int>(sizeof(ScheduleShared));
+  static constexpr int kTmemQ = 0, kTmemS = 128, kTmemO = 384;  // columns
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -105,10 +114,10 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
   }
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   auto bar = [&](int i) { return base + L::kBars + 8u * i; };
-  const uint32_t q_full = bar(0), s_full = bar(2), p_full = bar(4), o_full = bar(6);  // one per half
-  const uint32_t sc_full = bar(8), sc_empty = bar(10), it_full = bar(12), it_empty = bar(14);  // two stages
-  const uint32_t kv_full = bar(16), kv_empty = bar(16 + L::kRing);
-  static_assert(16 + 2 * L::kRing <= 32, "barriers");
+  const uint32_t q_full = bar(0), p_full = bar(1), o_full = bar(2);
+  const uint32_t s_full = bar(4), sc_full = bar(6), sc_empty = bar(8), it_full = bar(10), it_empty = bar(12);  // two each
+  const uint32_t kv_full = bar(14), kv_empty = bar(14 + L::kRing);
+  static_assert(14 + 2 * L::kRing <= L::kNumBars, "barriers");
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + L::kMisc);
   volatile uint32_t* abort_flag = misc + 1;
   volatile float* value_back = reinterpret_cast<volatile float*>(misc + 2);  // per scale stage
@@ -117,11 +126,11 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
   const Waiter wait{abort_flag, a.c.status, timeout_ns};
 
   if (tid == 0) {
+    ptx::mbar_init(q_full, 8);
+    ptx::mbar_init(p_full, 8);
+    ptx::mbar_init(o_full, 1);
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(q_full + 8 * i, 4);
       ptx::mbar_init(s_full + 8 * i, 1);
-      ptx::mbar_init(p_full + 8 * i, 4);
-      ptx::mbar_init(o_full + 8 * i, 1);
       ptx::mbar_init(sc_full + 8 * i, 1);
       ptx::mbar_init(sc_empty + 8 * i, 8);
       ptx::mbar_init(it_full + 8 * i, 1);
@@ -135,7 +144,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
     ptx::fence_mbar_init();
   }
   if (warp == 0) {
-    ptx::tmem_alloc<1>(base + L::kMisc, 512);  // S of both halves, O of both halves
+    ptx::tmem_alloc<1>(base + L::kMisc, 512);
     ptx::tmem_relinquish<1>();
   }
   ptx::tc_fence_before_sync();
@@ -163,90 +172,67 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
       if (!body(it)) return;
     }
   };
-  auto second_half = [](const Item& it) { return it.rows > it.tile * kManyRows + 128; };
 
   if (warp < 4) {
     ptx::setmaxnreg_dec<kRegsControl>();
     if (warp == 0) {
       // ======================= MMA issuer =======================
-      uint32_t kv_n = 0;             // ring buffers consumed
-      uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;  // phases per half
+      uint32_t kv_n = 0;  // ring buffers used by earlier items
+      uint32_t nb = 0;    // blocks of earlier items
+      uint32_t ni = 0;    // items
       constexpr uint32_t idesc_s = ptx::make_idesc(1u, 0u, 0u, 0u, 0u, 128u, 128u);
       constexpr uint32_t idesc_o = ptx::make_idesc(1u, 0u, 0u, 0u, 1u, 128u, static_cast<uint32_t>(DIM));
       for_items([&](const Item& it) {
-        const int halves = second_half(it) ? 2 : 1;
         const unsigned blocks = it.hi - it.lo;
         auto kv_wait = [&](uint32_t n) {
           return wait(kv_full + 8 * (n % L::kRing), (n / L::kRing) & 1u, TFCCB200_DEV_TIMEOUT_MMA);
         };
-        auto tile = [&](uint32_t n) { return base + L::kKv + (n % L::kRing) * L::kOperand; };
-        auto score = [&](int h, uint32_t n) {
+        auto tile = [&](uint32_t n) { return base + (n % L::kRing) * L::kOperand; };
+        // S of the item's block j, from ring buffer kv_n + 2 j
+        auto score = [&](unsigned j) {
+          const uint32_t n = kv_n + 2 * j, s2 = (nb + j) & 1u;
+          if (!kv_wait(n)) return false;
+          ptx::tc_fence_after_sync();
           if (lane == 0) {
             const uint32_t k = tile(n);
 #pragma unroll
-            for (int part = 1; part >= 0; --part) {  // the small terms first
-              const uint32_t q = base + L::kQ + (2 * h + part) * L::kOperand;
+            for (int part = 1; part >= 0; --part)  // the small terms first
 #pragma unroll
-              for (int s = 0; s < kSteps; ++s) {
-                const uint32_t off = (s >> 2) * kTileBytes + (s & 3) * 32;
-                ptx::umma<ptx::MmaKind::BF16, 1>(tmem + h * 128, ptx::smem_desc(q + off, 16, 1024, ptx::kLayoutSw128),
-                                                 ptx::smem_desc(k + off, 16, 1024, ptx::kLayoutSw128), idesc_s,
-                                                 (part == 1 && s == 0) ? 0u : 1u);
-              }
-            }
-            ptx::umma_commit<1>(s_full + 8 * h, 0);
+              for (int s = 0; s < kSteps; ++s)
+                ptx::umma_f16_ts(tmem + L::kTmemS + s2 * 128, tmem + L::kTmemQ + part * (DIM / 2) + s * 8,
+                                 ptx::smem_desc(k + (s >> 2) * kTileBytes + (s & 3) * 32, 16, 1024, ptx::kLayoutSw128),
+                                 idesc_s, (part == 1 && s == 0) ? 0u : 1u);
+            ptx::umma_commit<1>(s_full + 8 * s2, 0);
+            ptx::umma_commit<1>(kv_empty + 8 * (n % L::kRing), 0);
           }
           __syncwarp();
+          return true;
         };
-        auto weigh = [&](int h, uint32_t n) {
+        if (!wait(q_full, ni++ & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
+        if (!score(0)) return false;
+        for (unsigned j = 0; j < blocks; ++j) {
+          // The next block's S goes over the weights of the block before this one, whose products
+          // were issued earlier: one thread's MMAs run in the order of issue.
+          if (j + 1 < blocks && !score(j + 1)) return false;
+          const uint32_t n = kv_n + 2 * j + 1, s2 = (nb + j) & 1u;
+          if (!kv_wait(n) || !wait(p_full, (nb + j) & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
+          ptx::tc_fence_after_sync();
           if (lane == 0) {
             const uint32_t v = tile(n);
 #pragma unroll
             for (int part = 1; part >= 0; --part)
 #pragma unroll
               for (int s = 0; s < 8; ++s)
-                ptx::umma_f16_ts(tmem + 256 + h * 128, tmem + h * 128 + (s >> 1) * 32 + (s & 1) * 8 + part * 16,
+                ptx::umma_f16_ts(tmem + L::kTmemO, tmem + L::kTmemS + s2 * 128 + s * 16 + part * 8,
                                  ptx::smem_desc(v + s * 2048, kTileBytes, 1024, ptx::kLayoutSw128), idesc_o,
                                  (part == 1 && s == 0) ? 0u : 1u);
-            ptx::umma_commit<1>(o_full + 8 * h, 0);
+            ptx::umma_commit<1>(o_full, 0);
+            ptx::umma_commit<1>(kv_empty + 8 * (n % L::kRing), 0);
           }
           __syncwarp();
-        };
-        auto release = [&](uint32_t n) {
-          if (lane == 0) ptx::umma_commit<1>(kv_empty + 8 * (n % L::kRing), 0);
-          __syncwarp();
-        };
-        if (!wait(q_full, nq0++ & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
-        if (!kv_wait(kv_n)) return false;
-        ptx::tc_fence_after_sync();
-        score(0, kv_n);
-        if (halves == 2) {
-          if (!wait(q_full + 8, nq1++ & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
-          ptx::tc_fence_after_sync();
-          score(1, kv_n);
         }
-        release(kv_n);
-        for (unsigned j = 0; j < blocks; ++j) {
-          const uint32_t v = kv_n + 1, k = kv_n + 2;
-          const bool more = j + 1 < blocks;
-          for (int h = 0; h < halves; ++h) {
-            if (!wait(p_full + 8 * h, (h ? np1++ : np0++) & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
-            if (h == 0 && !kv_wait(v)) return false;
-            ptx::tc_fence_after_sync();
-            weigh(h, v);
-            if (h == halves - 1) release(v);
-            // S of the half's next block goes over the weights that the products just issued read:
-            // one thread's MMAs run in the order of issue
-            if (more) {
-              if (h == 0 && !kv_wait(k)) return false;
-              ptx::tc_fence_after_sync();
-              score(h, k);
-              if (h == halves - 1) release(k);
-            }
-          }
-          kv_n += more ? 2 : 1;
-        }
-        kv_n += 1;
+        kv_n += 2 * blocks;
+        nb += blocks;
         return true;
       });
     } else if (warp == 1) {
@@ -348,7 +334,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
       for (unsigned i = 0; i < tiles; ++i, ++n) {
         const unsigned s = n % L::kRing;
         if (!wait(kv_empty + 8 * s, ((n / L::kRing) & 1u) ^ 1u, TFCCB200_DEV_TIMEOUT_CONVERT)) return false;
-        uint8_t* dst = smem + L::kKv + s * L::kOperand;
+        uint8_t* dst = smem + s * L::kOperand;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const unsigned r = cw * 32 + g * 8 + r8;
@@ -373,181 +359,227 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
   } else {
     // ======================= softmax, sums, output =======================
     ptx::setmaxnreg_inc<kRegsSoftmax>();
-    const int h = static_cast<int>(warp >> 2) - 2;
-    const unsigned r = (warp & 3u) * 32 + lane;  // row of the half = lane of tensor memory
-    const uint32_t lane_addr = tmem + (((warp & 3u) * 32) << 16);
-    const uint32_t t_s = lane_addr + h * 128, t_o = lane_addr + 256 + h * 128;
-    uint32_t ns = 0, nb = 0;  // blocks of this half, blocks of the CTA
+    const unsigned g = lane >> 2, t = lane & 3u;
+    const unsigned lane0 = (warp & 3u) * 32 + ((warp >> 2) - 2) * 16;  // the warp's first row = lane of tensor memory
+    const uint32_t rows_addr = tmem + (lane0 << 16);
+    uint32_t nb = 0;  // blocks so far
     for_items([&](const Item& it) {
       const unsigned blocks = it.hi - it.lo;
-      if (h == 1 && !second_half(it)) {  // nothing to do, but the scale stages count on every warp
-        for (unsigned j = 0; j < blocks; ++j, ++nb) {
-          if (!wait(sc_full + 8 * (nb & 1u), (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(sc_empty + 8 * (nb & 1u));
-        }
-        return true;
-      }
-      const unsigned row = it.tile * kManyRows + h * 128 + r;
-      const bool live = row < it.rows;
-      const unsigned tok = live ? row / a.group : 0, hd = it.head * a.group + (live ? row % a.group : 0);
       const int past = it.length - it.count;
-      const int sees = !live ? 0 : (a.causal ? past + static_cast<int>(tok) + 1 : it.length);
-      // keys below this are seen by every row of the half
-      const int all_see = a.causal ? past + static_cast<int>((it.tile * kManyRows + h * 128) / a.group) + 1 : it.length;
+      // keys below this are seen by every row of the item
+      const int all_see = a.causal ? past + static_cast<int>(it.tile * kManyRows / a.group) + 1 : it.length;
+      float rs[2];  // of the thread's rows lane0 + g + 8 k: scale of the scores, visible keys
+      int sees[2];
 
-      // ---- the row of Q as two fp16 terms, scaled by a power of two ----
-      float row_scale;
+      // ---- Q as two fp16 terms, scaled by a power of two per row ----
       {
-        const float4* q = reinterpret_cast<const float4*>(
-            a.q + a.ldq * (static_cast<size_t>(it.first) + tok) + static_cast<size_t>(hd) * DIM);
-        uint32_t m = 0;
-        if (live) {
-#pragma unroll 8
-          for (int i = 0; i < DIM / 4; ++i) {
-            const float4 f = __ldg(q + i);
-            m = max(m, max(max(__float_as_uint(f.x * a.scale) & 0x7fffffffu, __float_as_uint(f.y * a.scale) & 0x7fffffffu),
-                           max(__float_as_uint(f.z * a.scale) & 0x7fffffffu, __float_as_uint(f.w * a.scale) & 0x7fffffffu)));
+        float f[2][DIM / 4];  // columns 8 i + 2 t, + 1
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const unsigned row = it.tile * kManyRows + lane0 + g + 8 * k;
+          const bool live = row < it.rows;
+          const unsigned tok = live ? row / a.group : 0, hd = it.head * a.group + (live ? row % a.group : 0);
+          sees[k] = !live ? 0 : (a.causal ? past + static_cast<int>(tok) + 1 : it.length);
+          const float2* q = reinterpret_cast<const float2*>(
+              a.q + a.ldq * (static_cast<size_t>(it.first) + tok) + static_cast<size_t>(hd) * DIM) + t;
+#pragma unroll
+          for (int i = 0; i < DIM / 8; ++i) {
+            const float2 x = live ? __ldg(q + 4 * i) : make_float2(0.f, 0.f);
+            f[k][2 * i] = x.x * a.scale;
+            f[k][2 * i + 1] = x.y * a.scale;
           }
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < DIM / 4; ++i) m = max(m, __float_as_uint(f[k][i]) & 0x7fffffffu);
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          // 2^(10 - exponent): the largest value lands in [2^10, 2^11); tiny rows take the bound of the
+          // range, a non-finite row 1 (it becomes NaN in any case)
+          const int ex = static_cast<int>(m >> 23) - 127;
+          const int sh = ex == 128 ? 0 : 10 - max(ex, -100);
+          const float up = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
+          rs[k] = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+#pragma unroll
+          for (int i = 0; i < DIM / 4; ++i) f[k][i] *= up;
         }
-        // 2^(10 - exponent): the largest value lands in [2^10, 2^11); tiny rows take the bound of the
-        // range, a non-finite row 1 (it becomes NaN in any case)
-        const int ex = static_cast<int>(m >> 23) - 127;
-        const int sh = ex == 128 ? 0 : 10 - max(ex, -100);
-        const float up = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
-        row_scale = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
-        uint8_t* hi = smem + L::kQ + 2 * h * L::kOperand + r * 128;
-        uint8_t* lo = hi + L::kOperand;
-#pragma unroll 4
-        for (int u = 0; u < DIM / 8; ++u) {  // 16-byte units of the operand row
-          float4 f = make_float4(0.f, 0.f, 0.f, 0.f), e = f;
-          if (live) f = __ldg(q + 2 * u), e = __ldg(q + 2 * u + 1);
-          // scaled in two steps, as the maximum was taken
-          const float x[8] = {f.x * a.scale * up, f.y * a.scale * up, f.z * a.scale * up, f.w * a.scale * up,
-                              e.x * a.scale * up, e.y * a.scale * up, e.z * a.scale * up, e.w * a.scale * up};
-          const unsigned off = (u >> 3) * kTileBytes + (((u & 7u) ^ (r & 7u)) << 4);
-          uint4 hh, ll;
-          hh.x = pack_half2(x[0], x[1]); hh.y = pack_half2(x[2], x[3]); hh.z = pack_half2(x[4], x[5]); hh.w = pack_half2(x[6], x[7]);
-          ll.x = pack_rest(x[0], x[1], hh.x); ll.y = pack_rest(x[2], x[3], hh.y);
-          ll.z = pack_rest(x[4], x[5], hh.z); ll.w = pack_rest(x[6], x[7], hh.w);
-          *reinterpret_cast<uint4*>(hi + off) = hh;
-          *reinterpret_cast<uint4*>(lo + off) = ll;
+#pragma unroll
+        for (int c = 0; c < DIM / 64; ++c) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float x = f[k][16 * c + 2 * i], y = f[k][16 * c + 2 * i + 1];
+              hi[2 * i + k] = pack_half2(x, y);
+              lo[2 * i + k] = pack_rest(x, y, hi[2 * i + k]);
+            }
+          ptx::tmem_st_16x32(rows_addr + L::kTmemQ + c * 32, hi);
+          ptx::tmem_st_16x32(rows_addr + L::kTmemQ + DIM / 2 + c * 32, lo);
         }
-        ptx::fence_proxy_async_smem();
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(q_full + 8 * h);
+        if (lane == 0) ptx::mbar_arrive(q_full);
       }
 
-      float o[DIM];
+      float o[DIM / 2];  // [4 i + 2 k + e]: column 8 i + 2 t + e of row k
 #pragma unroll
-      for (int i = 0; i < DIM; ++i) o[i] = 0.f;
-      float m = -INFINITY, l = 0.f, back = 0.f;
-      // adds the finished block's products (accumulated in tensor memory from zero) to o
+      for (int i = 0; i < DIM / 2; ++i) o[i] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float back[2] = {0.f, 0.f};  // what the products of the block to be drained are worth
+      // adds the products of the block before (accumulated in tensor memory from zero) to o
       auto drain = [&](uint32_t n) {
-        if (!wait(o_full + 8 * h, n & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
+        if (!wait(o_full, n & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         ptx::tc_fence_after_sync();
 #pragma unroll
-        for (int c = 0; c < DIM / 32; ++c) {
+        for (int c = 0; c < DIM / 64; ++c) {
           uint32_t x[32];
-          ptx::tmem_ld_32x32(t_o + c * 32, x);
+          ptx::tmem_ld_16x64(rows_addr + L::kTmemO + c * 64, x);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[c * 32 + i] = fmaf(__uint_as_float(x[i]), back, o[c * 32 + i]);
+          for (int i = 0; i < 32; i += 2) {
+            const float b = back[(i >> 1) & 1];
+            const float2 y = unpair(fma2(pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), pair(b, b),
+                                         pair(o[c * 32 + i], o[c * 32 + i + 1])));
+            o[c * 32 + i] = y.x;
+            o[c * 32 + i + 1] = y.y;
+          }
         }
         return true;
       };
-      for (unsigned j = 0; j < blocks; ++j, ++ns, ++nb) {
-        if (!wait(s_full + 8 * h, ns & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
-        ptx::tc_fence_after_sync();
-        if (j && !drain(ns - 1)) return false;
+      // One block; kMask: with keys that not every row sees (compiled apart: the comparisons would
+      // take more issue slots than the exponentials).
+      auto block = [&](unsigned j, auto mask) {
+        constexpr bool kMask = decltype(mask)::value;
         const unsigned s = nb & 1u;
+        const uint32_t t_s = rows_addr + L::kTmemS + s * 128;
+        // scales of this thread's keys 8 i + 2 t, + 1 in pairs, and (from 64 on) of their values
+        const uint64_t* scales = reinterpret_cast<const uint64_t*>(smem + L::kScales + s * 1024) + t;
         if (!wait(sc_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
-        const float4* ks = reinterpret_cast<const float4*>(smem + L::kScales + s * 1024);
-        const float4* vr = ks + 32;
-        back = value_back[s];
-        const int key0 = static_cast<int>((it.lo + j) * kBlockKeys);
-        const bool masked = key0 + static_cast<int>(kBlockKeys) > all_see;  // uniform in the half
-        // -- largest score of the row --
-        float top = -INFINITY;
+        if (!wait(s_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
+        ptx::tc_fence_after_sync();
+        const int first = static_cast<int>((it.lo + j) * kBlockKeys + 2 * t);  // the thread's first key
+        // -- scores times key scales, [4 i + 2 k + e]: key first + 8 i + e of row k --
+        float y[64];
+        float top[2] = {-INFINITY, -INFINITY};
+        ptx::tmem_ld_16x64(t_s, reinterpret_cast<uint32_t(&)[32]>(y[0]));
+        ptx::tmem_ld_16x64(t_s + 64, reinterpret_cast<uint32_t(&)[32]>(y[32]));
+        ptx::tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          ptx::tmem_ld_32x32(t_s + c * 32, x);
-          ptx::tmem_ld_wait();
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t ks = scales[4 * i];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k = ks[c * 8 + i / 4];
-            const float y[4] = {__uint_as_float(x[i]) * k.x, __uint_as_float(x[i + 1]) * k.y,
-                                __uint_as_float(x[i + 2]) * k.z, __uint_as_float(x[i + 3]) * k.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!masked || key0 + c * 32 + i + e < sees) top = fmaxf(top, y[e]);
-          }
-        }
-        top *= row_scale;
-        const bool grows = top > m + kLazy;  // (true for the first finite one: m is -inf)
-        if (__any_sync(0xffffffffu, grows)) {
-          const float next = grows ? top : m;
-          const float f = exp2_fast(m - (next == -INFINITY ? 0.f : next));
-          m = next;
-          l *= f;
-#pragma unroll
-          for (int i = 0; i < DIM; ++i) o[i] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        // -- weights, as two terms over the scores they come from --
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          ptx::tmem_ld_32x32(t_s + c * 32, x);
-          ptx::tmem_ld_wait();
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k = ks[c * 8 + i / 4], v = vr[c * 8 + i / 4];
-            float p[4] = {exp2_fast(fmaf(__uint_as_float(x[i]) * k.x, row_scale, -ref)),
-                          exp2_fast(fmaf(__uint_as_float(x[i + 1]) * k.y, row_scale, -ref)),
-                          exp2_fast(fmaf(__uint_as_float(x[i + 2]) * k.z, row_scale, -ref)),
-                          exp2_fast(fmaf(__uint_as_float(x[i + 3]) * k.w, row_scale, -ref))};
-            float y[4] = {p[0] * v.x, p[1] * v.y, p[2] * v.z, p[3] * v.w};
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (key0 + c * 32 + i + e >= sees) p[e] = y[e] = 0.f;
+          for (int k = 0; k < 2; ++k) {
+            float* e = &y[4 * i + 2 * k];
+            float2 u = unpair(mul2(pair(e[0], e[1]), ks));
+            if constexpr (kMask) {
+              u.x = first + 8 * i < sees[k] ? u.x : -INFINITY;
+              u.y = first + 8 * i + 1 < sees[k] ? u.y : -INFINITY;
             }
-            l += (p[0] + p[1]) + (p[2] + p[3]);
-            w[i / 2] = pack_half2(y[0], y[1]);
-            w[i / 2 + 1] = pack_half2(y[2], y[3]);
-            w[16 + i / 2] = pack_rest(y[0], y[1], w[i / 2]);
-            w[16 + i / 2 + 1] = pack_rest(y[2], y[3], w[i / 2 + 1]);
+            e[0] = u.x;
+            e[1] = u.y;
+            top[k] = fmaxf(top[k], fmaxf(u.x, u.y));
           }
-          ptx::tmem_st_32x32(t_s + c * 32, w);
         }
+        bool grows = false;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+          top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2)) * rs[k];
+          grows |= top[k] > m[k] + kLazy;  // (true for the first finite one: m is -inf)
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float next = top[k] > m[k] + kLazy ? top[k] : m[k];
+            const float f = exp2_fast(m[k] - (next == -INFINITY ? 0.f : next));
+            m[k] = next;
+            l[k] *= f;
+            back[k] *= f;
+#pragma unroll
+            for (int i = 0; i < DIM / 8; ++i) {
+              o[4 * i + 2 * k] *= f;
+              o[4 * i + 2 * k + 1] *= f;
+            }
+          }
+        }
+        // -- weights, as two terms over the scores they come from: 16 scores become 8 columns of hi
+        // and 8 of lo terms --
+        const uint64_t rs2[2] = {pair(rs[0], rs[0]), pair(rs[1], rs[1])};
+        const float r0 = m[0] == -INFINITY ? 0.f : -m[0], r1 = m[1] == -INFINITY ? 0.f : -m[1];
+        const uint64_t ref2[2] = {pair(r0, r0), pair(r1, r1)};
+        uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {  // 32 keys at a time
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = 4 * ch + i;
+            const uint64_t vs = scales[64 + 4 * c];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float2 e = unpair(fma2(pair(y[4 * c + 2 * k], y[4 * c + 2 * k + 1]), rs2[k], ref2[k]));
+              const uint64_t p = pair(exp2_fast(e.x), exp2_fast(e.y));
+              l2[k] = add2(l2[k], p);
+              float2 u = unpair(mul2(p, vs));
+              if constexpr (kMask) {  // (0 * NaN)
+                u.x = first + 8 * c < sees[k] ? u.x : 0.f;
+                u.y = first + 8 * c + 1 < sees[k] ? u.y : 0.f;
+              }
+              // keys 8 c + 2 t, + 1: column 4 (c % 2) + t of the group c / 2 of 16 columns; lo 8 further
+              const uint32_t hi = pack_half2(u.x, u.y);
+              w[2 * (4 * (i >> 1) + (i & 1)) + k] = hi;
+              w[2 * (4 * (i >> 1) + 2 + (i & 1)) + k] = pack_rest(u.x, u.y, hi);
+            }
+          }
+          ptx::tmem_st_16x32(t_s + ch * 32, w);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 f = unpair(l2[k]);
+          l[k] += f.x + f.y;
+        }
+        if (j && !drain(nb - 1)) return false;
+        back[0] = back[1] = value_back[s];
         ptx::tmem_st_wait();
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
           ptx::mbar_arrive(sc_empty + 8 * s);
-          ptx::mbar_arrive(p_full + 8 * h);
+          ptx::mbar_arrive(p_full);
         }
+        return true;
+      };
+      for (unsigned j = 0; j < blocks; ++j, ++nb) {
+        const bool masked = static_cast<int>((it.lo + j + 1) * kBlockKeys) > all_see;  // the same in all rows
+        if (!(masked ? block(j, std::true_type()) : block(j, std::false_type()))) return false;
       }
-      if (!drain(ns - 1)) return false;
-      if (!live) return true;
-      if (it.whole) {
-        const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;  // nothing seen: 0
-        float4* dst = reinterpret_cast<float4*>(a.out + a.ldo * (static_cast<size_t>(it.first) + tok) +
-                                                static_cast<size_t>(hd) * DIM);
+      if (!drain(nb - 1)) return false;
+
+      float* const part = it.whole ? nullptr : piece<kManyRows, DIM>(a, blockIdx.x, it.lo == 0);
 #pragma unroll
-        for (int i = 0; i < DIM; i += 4)
-          dst[i / 4] = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-      } else {
-        float* p = piece<kManyRows, DIM>(a, blockIdx.x, it.lo == 0);
-        const unsigned pr = h * 128 + r;
-        p[pr] = m;
-        p[kManyRows + pr] = l;
-        float4* dst = reinterpret_cast<float4*>(p + 2 * kManyRows + pr * DIM);
+      for (int k = 0; k < 2; ++k) {
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+        const unsigned r = lane0 + g + 8 * k, row = it.tile * kManyRows + r;
+        if (row < it.rows) {
+          float inv = 1.f;
+          float* dst;
+          if (part) {
+            if (t == 0) {
+              part[r] = m[k];
+              part[kManyRows + r] = l[k];
+            }
+            dst = part + 2 * kManyRows + r * DIM + 2 * t;
+          } else {
+            inv = m[k] == -INFINITY && l[k] == 0.f ? 0.f : 1.f / l[k];  // nothing seen: 0
+            dst = a.out + a.ldo * (static_cast<size_t>(it.first) + row / a.group) +
+                  (static_cast<size_t>(it.head) * a.group + row % a.group) * DIM + 2 * t;
+          }
 #pragma unroll
-        for (int i = 0; i < DIM; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < DIM / 8; ++i)
+            *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[4 * i + 2 * k] * inv, o[4 * i + 2 * k + 1] * inv);
+        }
       }
       return true;
     });
