@@ -193,15 +193,18 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           const uint32_t n = kv_n + 2 * j, s2 = (nb + j) & 1u;
           if (!kv_wait(n)) return false;
           ptx::tc_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t k = tile(n);
+          __syncwarp();
+          if (ptx::elect_one()) {
+            const uint64_t desc = ptx::smem_desc(tile(n), 16, 1024, ptx::kLayoutSw128);
+            const uint32_t lo = static_cast<uint32_t>(desc), hi = static_cast<uint32_t>(desc >> 32);
+            const uint32_t d = tmem + L::kTmemS + s2 * 128, q = tmem + L::kTmemQ;
+            ptx::umma_f16_ts<false>(d, q + DIM / 2, lo, hi, idesc_s);  // the small terms first
 #pragma unroll
-            for (int part = 1; part >= 0; --part)  // the small terms first
+            for (int s = 1; s < kSteps; ++s)
+              ptx::umma_f16_ts<true>(d, q + DIM / 2 + s * 8, lo + ((s >> 2) * kTileBytes + (s & 3) * 32) / 16, hi, idesc_s);
 #pragma unroll
-              for (int s = 0; s < kSteps; ++s)
-                ptx::umma_f16_ts(tmem + L::kTmemS + s2 * 128, tmem + L::kTmemQ + part * (DIM / 2) + s * 8,
-                                 ptx::smem_desc(k + (s >> 2) * kTileBytes + (s & 3) * 32, 16, 1024, ptx::kLayoutSw128),
-                                 idesc_s, (part == 1 && s == 0) ? 0u : 1u);
+            for (int s = 0; s < kSteps; ++s)
+              ptx::umma_f16_ts<true>(d, q + s * 8, lo + ((s >> 2) * kTileBytes + (s & 3) * 32) / 16, hi, idesc_s);
             ptx::umma_commit<1>(s_full + 8 * s2, 0);
             ptx::umma_commit<1>(kv_empty + 8 * (n % L::kRing), 0);
           }
@@ -217,15 +220,16 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           const uint32_t n = kv_n + 2 * j + 1, s2 = (nb + j) & 1u;
           if (!kv_wait(n) || !wait(p_full, (nb + j) & 1u, TFCCB200_DEV_TIMEOUT_MMA)) return false;
           ptx::tc_fence_after_sync();
-          if (lane == 0) {
-            const uint32_t v = tile(n);
+          __syncwarp();
+          if (ptx::elect_one()) {
+            const uint64_t desc = ptx::smem_desc(tile(n), kTileBytes, 1024, ptx::kLayoutSw128);
+            const uint32_t lo = static_cast<uint32_t>(desc), hi = static_cast<uint32_t>(desc >> 32);
+            const uint32_t d = tmem + L::kTmemO, p = tmem + L::kTmemS + s2 * 128;
+            ptx::umma_f16_ts<false>(d, p + 8, lo, hi, idesc_o);
 #pragma unroll
-            for (int part = 1; part >= 0; --part)
+            for (int s = 1; s < 8; ++s) ptx::umma_f16_ts<true>(d, p + s * 16 + 8, lo + s * (2048 / 16), hi, idesc_o);
 #pragma unroll
-              for (int s = 0; s < 8; ++s)
-                ptx::umma_f16_ts(tmem + L::kTmemO, tmem + L::kTmemS + s2 * 128 + s * 16 + part * 8,
-                                 ptx::smem_desc(v + s * 2048, kTileBytes, 1024, ptx::kLayoutSw128), idesc_o,
-                                 (part == 1 && s == 0) ? 0u : 1u);
+            for (int s = 0; s < 8; ++s) ptx::umma_f16_ts<true>(d, p + s * 16, lo + s * (2048 / 16), hi, idesc_o);
             ptx::umma_commit<1>(o_full, 0);
             ptx::umma_commit<1>(kv_empty + 8 * (n % L::kRing), 0);
           }
