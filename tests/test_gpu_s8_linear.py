@@ -139,6 +139,26 @@ def test_product(pkg, m, k, n, path):
     pkg.session.get_session(dev()).sync()
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 16, 16), (1, 5, 3), (3, 33, 130), (16, 768, 768), (8, 1003, 129), (16, 4096, 300), (9, 2000, 1),
+                                   (2, 300, 20000)])
+def test_few_tokens(pkg, m, k, n):
+    a, sa, b, sb, bias = operands(m, k, n, m + k)
+    check(pkg.quantization.matmul_scaled(a, sa, b, sb, path="skinny"), a, sa, b, sb, None)
+    check(pkg.quantization.matmul_scaled(a, sa, b, sb, bias, activation="gelu", path="skinny"), a, sa, b, sb, bias, True)
+
+
+def test_nothing_behind_the_operands_is_touched(pkg):
+    """Operands that end where their allocation ends, the last row shorter than the pitch: the product may not
+    depend on, or read, what would follow (a slice of a packed weight)."""
+    wide = torch.randint(-127, 128, (200, 512), dtype=torch.int8, device=dev())
+    w = wide[:, 512 - 112 - 32:512 - 32]  # 112 columns, pitch 512
+    tall = torch.randint(-127, 128, (30, 256), dtype=torch.int8, device=dev())
+    x = tall[:, 48:48 + 200]              # K = 200, pitch 256
+    sa, sb = torch.rand(30, device=dev()), torch.rand(112, device=dev())
+    for rows in (1, 16, 30):
+        check(pkg.quantization.matmul_scaled(x[:rows], sa[:rows].contiguous(), w, sb), x[:rows], sa[:rows], w, sb, None)
+
+
 @pytest.mark.parametrize("m,k,n", [(5, 63, 61), (70, 130, 100), (1, 1, 1), (200, 33, 17)])
 def test_product_of_unaligned_operands(pkg, m, k, n):
     a, sa, b, sb, bias = operands(m, k, n, m, pad=False)

@@ -18,7 +18,7 @@ def linear_args(**kw):
 @pytest.mark.parametrize("kw,want", [
     ({"A": None}, EINVAL), ({"B": None}, EINVAL), ({"C": None}, EINVAL), ({"sa": None}, EINVAL), ({"sb": None}, EINVAL),
     ({"M": 0}, EINVAL), ({"N": 0}, EINVAL), ({"K": 0}, EINVAL), ({"lda": 63}, EINVAL), ({"ldb": 63}, EINVAL),
-    ({"act": 7}, EINVAL), ({"path": 9}, EINVAL), ({"path": 2}, EINVAL), ({"K": 133001, "lda": 133008}, EOVERFLOW),
+    ({"act": 7}, EINVAL), ({"path": 9}, EINVAL), ({"path": 2, "M": 17}, EUNSUPPORTED), ({"path": 2, "lda": 72}, EUNSUPPORTED), ({"K": 133001, "lda": 133008}, EOVERFLOW),
     ({"M": 1 << 20, "N": 1 << 13, "ldb": 1 << 13}, EOVERFLOW), ({"C": P + 2}, EALIGN), ({"sa": P + 1}, EALIGN),
     ({"bias": P + 2}, EALIGN), ({"path": 3, "lda": 72}, EUNSUPPORTED), ({"path": 4, "B": P + 4}, EUNSUPPORTED)])
 def test_product_refusals(pkg, kw, want):

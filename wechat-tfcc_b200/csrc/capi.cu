@@ -845,7 +845,10 @@ int run_s8_gemm(const S8GemmArgs& a, int path) {
   if (misaligned(a.C, 4) || misaligned(a.a_scales, 4) || misaligned(a.b_scales, 4) || misaligned(a.bias, 4))
     return TFCCB200_EALIGN;
   switch (path) {
-    case TFCCB200_PATH_AUTO: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, -1) : simt_s8_gemm(a);
+    case TFCCB200_PATH_AUTO:
+      if (few_s8_gemm_supported(a)) return few_s8_gemm(a);
+      return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, -1) : simt_s8_gemm(a);
+    case TFCCB200_PATH_SKINNY: return few_s8_gemm_supported(a) ? few_s8_gemm(a) : TFCCB200_EUNSUPPORTED;
     case TFCCB200_PATH_SIMT: return simt_s8_gemm(a);
     case TFCCB200_PATH_UMMA: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 0) : TFCCB200_EUNSUPPORTED;
     case TFCCB200_PATH_UMMA2: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 1) : TFCCB200_EUNSUPPORTED;

@@ -222,6 +222,8 @@ struct S8GemmArgs {
 int quantize_tokens(cudaStream_t stream, const float* src, unsigned long long ld_src, unsigned rows,
                     unsigned cols, int8_t* codes, unsigned long long ld_codes, float* scales);
 int simt_s8_gemm(const S8GemmArgs& a);
+bool few_s8_gemm_supported(const S8GemmArgs& a);  // M <= 16
+int few_s8_gemm(const S8GemmArgs& a);
 bool umma_s8_gemm_supported(const S8GemmArgs& a);
 int umma_s8_gemm(const S8GemmArgs& a, int force_pair);  // force_pair: -1 = choose
 

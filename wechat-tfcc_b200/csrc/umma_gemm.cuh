@@ -193,8 +193,10 @@ struct UmmaGemmConfig {
   static constexpr int kEpiStagingBytes = kNumEpilogueWarps * kEpiStageBytes;
   static constexpr int kBarrierBytes =
       256 + 16 * kMaxSkSegments + 16 + 128;  // + segment table, store target
+  // S8: scale and bias of the tile's columns, a copy per epilogue warp
+  static constexpr int kColTermBytes = kKind == ptx::MmaKind::S8 ? kNumEpilogueWarps * 2 * BN * 4 : 0;
   static constexpr int kSmemBytes =
-      kRingBytes + kEpiStagingBytes + kBarrierBytes + 1024;  // +align slack
+      kRingBytes + kEpiStagingBytes + kBarrierBytes + kColTermBytes + 1024;  // +align slack
   static constexpr uint32_t kIdesc =
       (kKind == ptx::MmaKind::TF32)
           ? ptx::make_idesc(1u, 2u, 2u, 0u, 1u, static_cast<uint32_t>(kTileM), BN)
@@ -957,17 +959,30 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
             row_term += static_cast<uint32_t>(__ldg(p.rsA + static_cast<size_t>(p.strideRsA) * b + row)) * ob;
         }
         float row_scale = 0.f;
-        if constexpr (kKind == ptx::MmaKind::S8) row_scale = row_ok ? __ldg(p.a_scales + row) : 0.f;
+        float* const terms = reinterpret_cast<float*>(bar_gen + Cfg::kBarrierBytes) + (warp - Cfg::kFirstEpilogueWarp) * 2 * BN;
+        if constexpr (kKind == ptx::MmaKind::S8) {
+          // the tile's row and column factors, fetched while the mainloop runs
+          row_scale = row_ok ? __ldg(p.a_scales + row) : 0.f;
+          if (row0 < pM) {
+            for (unsigned i = lane; i < BN; i += 32) {
+              const unsigned col = col0 + i;
+              terms[i] = col < pN ? __ldg(p.b_scales + col) : 0.f;
+              terms[BN + i] = (pbias && col < pN) ? __ldg(pbias + col) : 0.f;
+            }
+          }
+          __syncwarp();
+        }
         bounded_wait<false>(tmem_full(acc), acc_ph, TFCCB200_DEV_TIMEOUT_EPILOGUE, ctl);
         ptx::tc_fence_after_sync();
         const uint32_t taddr = lane_addr + acc * BN;
         const EpiTarget& tgt = *tgt_smem;
         if constexpr (kKind == ptx::MmaKind::S8) {
           // fp32 results from the exact int32 sums: one column block of 32 after the other goes
-          // through the warp's staging block, which all four warps of the quarter keep for
-          // themselves, and leaves by TMA store (or, for rows that are no multiple of 16 bytes, by
-          // 128-byte row segments).
+          // through a staging block of the warp and leaves by TMA store (or, for rows that are no
+          // multiple of 16 bytes, by 128-byte row segments).  The CTA's last tile stages in the
+          // dead ring, all blocks side by side, so that no store waits for another.
           const int act = tgt.activation;
+          const bool last_tile = si + 1 == num_segments;
           unsigned c_lo = 0, c_hi = BN / 32;
           const uint4* red = nullptr;
           unsigned qper = 0, ew = warp - Cfg::kFirstEpilogueWarp;
@@ -1000,14 +1015,11 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
             c_lo = krank * (slice / 32);
             c_hi = c_lo + slice / 32;
           }
+          if (row0 >= pM) c_hi = c_lo;  // no row of this warp exists
 #pragma unroll 1
           for (unsigned c = c_lo; c < c_hi; ++c) {
             const unsigned colb = col0 + c * 32;
             if (colb >= pN) break;  // warp-uniform
-            // lane l keeps column l's scale and bias
-            const bool col_ok = colb + lane < pN;
-            const float my_scale = col_ok ? __ldg(p.b_scales + colb + lane) : 0.f;
-            const float my_bias = (pbias && col_ok) ? __ldg(pbias + colb + lane) : 0.f;
             uint32_t r[32];
             ptx::tmem_ld_32x32(taddr + c * 32, r);
             ptx::tmem_ld_wait();
@@ -1020,23 +1032,33 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
                 }
               }
             }
-            if (tgt.tma_store) epi_tma_stage_free(lane);
+            // (in a cluster the block overwrites the first source's part of this very block, which this
+            // warp alone reads and has just read)
+            uint32_t* const out = !last_tile ? stage_one
+                                  : reinterpret_cast<uint32_t*>(smem_gen) +
+                                        (red ? ew * (qper / 8) + (c - c_lo) : ew * (BN / 32) + c) * (Cfg::kEpiStageBytes / 4);
+            if (tgt.tma_store && !last_tile) epi_tma_stage_free(lane);
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float y = fmaf(static_cast<float>(static_cast<int>(r[j])) * row_scale,
-                                   __shfl_sync(0xffffffffu, my_scale, j), __shfl_sync(0xffffffffu, my_bias, j));
-              r[j] = __float_as_uint(act != TFCCB200_ACT_NONE ? apply_activation(y, act) : y);
+            for (int qq = 0; qq < 8; ++qq) {
+              const float4 sc = *reinterpret_cast<const float4*>(terms + c * 32 + 4 * qq);
+              const float4 bi = *reinterpret_cast<const float4*>(terms + BN + c * 32 + 4 * qq);
+              const float s4[4] = {sc.x, sc.y, sc.z, sc.w}, b4[4] = {bi.x, bi.y, bi.z, bi.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y = fmaf(static_cast<float>(static_cast<int>(r[4 * qq + e])) * row_scale, s4[e], b4[e]);
+                r[4 * qq + e] = __float_as_uint(act == TFCCB200_ACT_GELU_ERF ? gelu_erfc(y) : y);
+              }
+              epi_stage_chunk(out, lane, qq, make_uint4(r[4 * qq], r[4 * qq + 1], r[4 * qq + 2], r[4 * qq + 3]));
             }
-#pragma unroll
-            for (int qq = 0; qq < 8; ++qq)
-              epi_stage_chunk(stage, lane, qq, make_uint4(r[4 * qq], r[4 * qq + 1], r[4 * qq + 2], r[4 * qq + 3]));
             if (tgt.tma_store) {
-              epi_tma_store_block(stage, lane, &tmapC, colb, row0, b);
+              epi_tma_store_block(out, lane, &tmapC, colb, row0, b);
             } else {
               __syncwarp();
+              const bool col_ok = colb + lane < pN;
 #pragma unroll 4
               for (unsigned rr = 0; rr < 32; ++rr) {
-                const uint32_t v = stage[rr * 32 + (((lane >> 2) ^ (rr & 7u)) << 2) + (lane & 3u)];
+                const uint32_t v = out[rr * 32 + (((lane >> 2) ^ (rr & 7u)) << 2) + (lane & 3u)];
                 if (row0 + rr < pM && col_ok)
                   tgt.dst[0][static_cast<unsigned long long>(row0 + rr) * tgt.ldc + colb + lane] = v;
               }
