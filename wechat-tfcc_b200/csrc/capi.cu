@@ -937,6 +937,7 @@ int tfccb200_qlinear_f32(void* stream, const float* x, size_t ldx, const int8_t*
   if (activation != TFCCB200_ACT_NONE && activation != TFCCB200_ACT_GELU_ERF) return TFCCB200_EINVAL;
   if (K > 133000u || shape_overflows(M, N, K, 1)) return TFCCB200_EOVERFLOW;
   const int st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
+  a.early_weights = true;
   return st != TFCCB200_OK ? st : run_s8_gemm(a, TFCCB200_PATH_AUTO);
 }
 

@@ -217,6 +217,10 @@ struct S8GemmArgs {
   unsigned long long lda, ldb;
   unsigned M, N, K;
   int activation;
+  // The kernel ahead in the stream is quantize_tokens, which lets its successor start only after
+  // everything before itself is complete: B, b_scales and bias may be read at once, only the codes
+  // and their scales have to be waited for.
+  bool early_weights;
   int* status;
 };
 int quantize_tokens(cudaStream_t stream, const float* src, unsigned long long ld_src, unsigned rows,

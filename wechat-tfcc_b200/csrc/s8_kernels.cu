@@ -2,6 +2,8 @@
 // and the product for operands the tensor-core path cannot take.
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "act.cuh"
 #include "internal.h"
 #include "pdl.cuh"
@@ -24,8 +26,10 @@ quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src,
   constexpr int kHold = 4;
   constexpr int kBlock = THREADS < 128 ? 128 : THREADS;
   __shared__ uint32_t sh[kBlock / 32];
-  pdl_release();
+  // In this order: once the next kernel may start, everything before this one is complete, and the
+  // product that follows can begin with its weights (S8GemmArgs::early_weights).
   pdl_wait();
+  pdl_release();
   const unsigned t = threadIdx.x % THREADS;
   const unsigned long long row = static_cast<unsigned long long>(blockIdx.x) * (kBlock / THREADS) + threadIdx.x / THREADS;
   const bool live = row < rows;
@@ -73,22 +77,27 @@ quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src,
 // ---- few tokens: memory-bound on the weights ------------------------------------------------------
 //
 // Up to 16 tokens against W [K, N]: a CTA takes 128 columns and a share of K, its eight warps deal the
-// share out in steps of 32 rows.  A lane reads 16 bytes of each of 8 rows straight into
-// registers (whole 128-byte lines per row over the warp, two steps in flight); a byte transposition
-// turns four rows into mma.sync m16n8k32 operands, whose columns may come in any order: lane group g
-// holds columns 16 g .. 16 g + 15, column j of each for the j-th product.  With the tokens as rows the
-// products cost 16 instructions per 4 KB of weights.  The int32 sums of the warps meet in shared memory and
-// those of a K split in the shared memory of a thread-block cluster; integer sums are exact in any order.
-// The tcgen05 kernel pads 16 tokens to 128 rows and leaves its epilogue to one warp per tile
-// (16x4096x16384 with GELU: 43 us).
+// share out in steps of 32 rows.  Each warp brings its steps (32 x 128 weights, 16 x 32 codes)
+// through a cp.async ring of its own, five stages deep: about 180 KB in flight per SM, which the
+// latency of memory asks for, without holding registers.  A lane reads 16 bytes of each of 8 rows; a byte
+// transposition turns four rows into mma.sync m16n8k32 operands, whose columns may come in any
+// order: lane group g holds columns 16 g .. 16 g + 15, column j of each for the j-th product.  With
+// the tokens as rows the products cost 16 instructions per 4 KB of weights.  The int32 sums of the warps
+// meet in shared memory and those of a K split in the shared memory of a thread-block cluster;
+// integer sums are exact in any order.  (The tcgen05 kernel pads 16 tokens to 128 rows and
+// leaves its epilogue to one warp per tile: 43 us for 16x4096x16384 with GELU; two steps
+// held in registers instead of the ring: 21 us.)
 constexpr int kFewThreads = 256;
 constexpr int kFewCols = 128;
 constexpr int kFewPitch = kFewCols + 12;  // ints per token in shared memory: rows start 12 banks apart
+constexpr int kFewStages = 5;
+constexpr int kFewStageBytes = 32 * kFewCols + 16 * 32;
+constexpr int kFewSmem = 8 * kFewStages * kFewStageBytes + 16 * kFewPitch * 4;
 
-struct FewStep {
-  uint4 w[8];     // rows 4 t + i and (from 4 on) 16 + 4 t + i of the step, 16 columns
-  uint32_t a[4];  // codes of tokens g and g + 8 in the product's operand order
-};
+// 16 bytes of which the first `live` exist (the rest arrives as zeros).
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live) : "memory");
+}
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -108,91 +117,95 @@ __device__ __forceinline__ void transpose4(const uint32_t (&r)[4], uint32_t (&c)
   c[3] = __byte_perm(x1, y1, 0x7632);
 }
 
-__global__ void __launch_bounds__(kFewThreads, 1) s8_few_kernel(const __grid_constant__ S8GemmArgs a, unsigned splits) {
-  __shared__ int sums[16 * kFewPitch];
+__global__ void __launch_bounds__(kFewThreads, 1)
+s8_few_kernel(const __grid_constant__ S8GemmArgs a, unsigned splits) {
+  extern __shared__ __align__(128) uint8_t few_smem[];
+  int* const sums = reinterpret_cast<int*>(few_smem + 8 * kFewStages * kFewStageBytes);
   pdl_release();
   const unsigned tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
   const unsigned rank = blockIdx.x % splits;
   const unsigned col0 = blockIdx.x / splits * kFewCols;
   const unsigned steps = (a.K + 31) / 32, per = (steps + splits - 1) / splits;
-  const unsigned first = rank * per, last = min(steps, first + per);  // this CTA's steps
-  for (unsigned i = tid; i < 16 * kFewPitch; i += kFewThreads) sums[i] = 0;
-  pdl_wait();
+  const unsigned first = min(steps, rank * per), last = min(steps, first + per);  // this CTA's steps
+  const uint8_t* const ring = few_smem + warp * kFewStages * kFewStageBytes;
+  const uint32_t ring_addr = ptx::smem_u32(ring);
 
-  const unsigned col = col0 + 16 * g;
-  const int8_t* const wp = a.B + col;
-  const int cols = static_cast<int>(a.N) - static_cast<int>(col);  // of the lane's 16 columns, those that exist
-  auto load = [&](unsigned step, FewStep& f) {
+  // 16-byte chunk c of row r of a step lies at chunk c ^ (r / 4 % 4 * 2): the four rows and two chunks
+  // that a quarter of a warp reads together then differ in their banks.
+  auto load_weights = [&](unsigned step, unsigned st) {
+    const unsigned c = lane & 7u, col = col0 + c * 16;
+    const int live = min(16, max(0, static_cast<int>(a.N) - static_cast<int>(col)));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned k = step * 32 + (i >> 2) * 16 + 4 * t + (i & 3);
-      f.w[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (k < a.K && cols > 0) {
-        const int8_t* p = wp + k * a.ldb;
-        if (cols >= 16) {
-          asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(f.w[i].x), "=r"(f.w[i].y), "=r"(f.w[i].z), "=r"(f.w[i].w)
-                       : "l"(p));
-        } else {  // the ragged end: only what exists is touched
-          uint32_t v[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (4 * q + 4 <= cols) {
-              v[q] = __ldg(reinterpret_cast<const uint32_t*>(p) + q);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 3; ++e)
-                if (4 * q + e < cols) v[q] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(p + 4 * q + e))) << (8 * e);
-            }
-          }
-          f.w[i] = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned m = g + (i & 1) * 8, k = step * 32 + (i >> 1) * 16 + 4 * t;
-      const int8_t* p = a.A + m * a.lda + k;
-      f.a[i] = 0u;
-      if (m < a.M) {
-        if (k + 4 <= a.K) {
-          f.a[i] = __ldg(reinterpret_cast<const uint32_t*>(p));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (k + e < a.K) f.a[i] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(p + e))) << (8 * e);
-        }
-      }
+      const unsigned r = i * 4 + (lane >> 3), k = step * 32 + r;
+      const bool in = k < a.K && live > 0;
+      cp_async_16(ring_addr + st * kFewStageBytes + r * kFewCols + ((c ^ ((r >> 1) & 6u)) << 4),
+                  in ? a.B + k * a.ldb + col : a.B, in ? live : 0);
     }
   };
+  auto load_codes = [&](unsigned step, unsigned st) {
+    const unsigned m = lane >> 1, k = step * 32 + (lane & 1u) * 16;
+    const int live = m < a.M ? min(16, max(0, static_cast<int>(a.K) - static_cast<int>(k))) : 0;
+    cp_async_16(ring_addr + st * kFewStageBytes + 32 * kFewCols + lane * 16, live > 0 ? a.A + m * a.lda + k : a.A, live);
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // What comes before the wait for the kernel ahead may only read what that kernel does not write
+  // and what was complete when that kernel began: see S8GemmArgs::early_weights.
+  if (a.early_weights)
+    for (unsigned s = 0; s < kFewStages - 1; ++s)
+      if (first + warp + 8 * s < last) load_weights(first + warp + 8 * s, s);
+  for (unsigned i = tid; i < 16 * kFewPitch; i += kFewThreads) sums[i] = 0;
+  pdl_wait();
+  for (unsigned s = 0; s < kFewStages - 1; ++s) {
+    if (first + warp + 8 * s < last) {
+      if (!a.early_weights) load_weights(first + warp + 8 * s, s);
+      load_codes(first + warp + 8 * s, s);
+    }
+    commit();
+  }
+
   int acc[16][4];
 #pragma unroll
   for (int j = 0; j < 16; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[j][i] = 0;
-  auto use = [&](const FewStep& f) {
+  unsigned st = 0;
+  for (unsigned s = first + warp; s < last; s += 8) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+    __syncwarp();
+    const uint8_t* const stage = ring + st * kFewStageBytes;
+    {
+      const unsigned ahead = s + 8 * (kFewStages - 1), into = st == 0 ? kFewStages - 1 : st - 1;
+      if (ahead < last) {
+        load_weights(ahead, into);
+        load_codes(ahead, into);
+      }
+      commit();
+    }
+    if (++st == kFewStages) st = 0;
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // tokens g, g + 8, k = 4 t and 16 + 4 t
+      f[i] = *reinterpret_cast<const uint32_t*>(stage + 32 * kFewCols + (g + (i & 1) * 8) * 32 + (i >> 1) * 16 + 4 * t);
+    uint4 w[8];  // rows 4 t + i and (from 4 on) 16 + 4 t + i
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned r = (i >> 2) * 16 + 4 * t + (i & 3);
+      w[i] = *reinterpret_cast<const uint4*>(stage + r * kFewCols + ((g ^ ((r >> 1) & 6u)) << 4));
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const uint32_t r0[4] = {(&f.w[0].x)[q], (&f.w[1].x)[q], (&f.w[2].x)[q], (&f.w[3].x)[q]};
-      const uint32_t r1[4] = {(&f.w[4].x)[q], (&f.w[5].x)[q], (&f.w[6].x)[q], (&f.w[7].x)[q]};
+      const uint32_t r0[4] = {(&w[0].x)[q], (&w[1].x)[q], (&w[2].x)[q], (&w[3].x)[q]};
+      const uint32_t r1[4] = {(&w[4].x)[q], (&w[5].x)[q], (&w[6].x)[q], (&w[7].x)[q]};
       uint32_t c0[4], c1[4];
       transpose4(r0, c0);
       transpose4(r1, c1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mma_s8(acc[4 * q + e], f.a, c0[e], c1[e]);
+      for (int e = 0; e < 4; ++e) mma_s8(acc[4 * q + e], f, c0[e], c1[e]);
     }
-  };
-  {
-    FewStep f0, f1;
-    unsigned s = first + warp;
-    if (s < last) load(s, f0);
-    for (; s < last; s += 16) {
-      if (s + 8 < last) load(s + 8, f1);
-      use(f0);
-      if (s + 16 < last) load(s + 16, f0);
-      if (s + 8 < last) use(f1);
-    }
+    __syncwarp();  // the stage may be overwritten
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   // column 16 n + j of the tile lies at place 8 j + n
   if (first + warp < last) {
@@ -306,12 +319,23 @@ int few_s8_gemm(const S8GemmArgs& a) {
   const DeviceInfo* di = current_device_info(&ce);
   if (!di) return static_cast<int>(ce);
   const unsigned tiles = (a.N + kFewCols - 1) / kFewCols, steps = (a.K + 31) / 32;
+  static std::atomic<unsigned long long> configured{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(s8_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured.fetch_or(bit, std::memory_order_release);
+  }
   // One CTA per SM: K is split while the CTAs still fit and every warp keeps a step of its own.
   unsigned splits = 1;
   while (splits < 8 && tiles * splits * 2 <= static_cast<unsigned>(di->sm_count) && steps >= splits * 2 * 8) splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * splits);
   cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = kFewSmem;
   cfg.stream = a.stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -322,7 +346,7 @@ int few_s8_gemm(const S8GemmArgs& a) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, s8_few_kernel, a, splits);
+  e = cudaLaunchKernelEx(&cfg, s8_few_kernel, a, splits);
   if (e != cudaSuccess) return static_cast<int>(e);
   count_launch();
   return TFCCB200_OK;
