@@ -105,7 +105,9 @@ class _Lib:
     def __getattr__(self, name):
         if self._dll is None:
             self._load()
-        return getattr(self._dll, name)
+        fn = getattr(self._dll, name)
+        setattr(self, name, fn)  # found directly from now on
+        return fn
 
 
 lib = _Lib()

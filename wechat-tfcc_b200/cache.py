@@ -23,7 +23,7 @@ import torch
 
 from . import exceptions
 from ._lib import check, lib
-from .session import get_session
+from .session import launch_context
 
 
 class _Struct(C.Structure):  # tfccb200_cache of include/tfcc_b200.h
@@ -38,7 +38,7 @@ class PagedCache:
     ``dim`` is 64 or 128, ``page_size`` a power of two up to 1024."""
 
     __slots__ = ("keys", "key_scales", "values", "value_scales", "pages", "kv_heads", "page_size", "dim",
-                 "device", "_struct")
+                 "device", "_struct", "_ref")
 
     def __init__(self, keys: torch.Tensor, key_scales: torch.Tensor, values: torch.Tensor,
                  value_scales: torch.Tensor):
@@ -64,6 +64,7 @@ class PagedCache:
         self.device = device
         self._struct = _Struct(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(),
                                self.pages, self.page_size, self.kv_heads, self.dim)
+        self._ref = C.byref(self._struct)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, device) -> "PagedCache":
@@ -78,9 +79,10 @@ def _sequences(cache, starts, lengths, table):
     """(starts, lengths, table pointers, batch, table width) of a call, checked."""
     if not isinstance(cache, PagedCache):
         raise exceptions.InvalidArgumentError("cache must be a PagedCache")
+    device = cache.device
     for t, name, rank in ((starts, "starts", 1), (lengths, "lengths", 1), (table, "table", 2)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != rank or t.numel() == 0 or \
-                t.device != cache.device or not t.is_contiguous():
+                t.device != device or not t.is_contiguous():
             raise exceptions.InvalidArgumentError(f"{name}: expected a contiguous int32 tensor of rank {rank} on {cache.device}")
     batch = lengths.shape[0]
     if starts.shape[0] != batch + 1 or table.shape[0] != batch:
@@ -109,9 +111,9 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Te
     cols = cache.kv_heads * cache.dim
     ldk = _packed(k, "k", None, cols, cache.device)
     ldv = _packed(v, "v", k.shape[0], cols, cache.device)
-    sess = get_session(cache.device)
-    with torch.cuda.device(cache.device):
-        check(lib.tfccb200_cache_append_f32(sess.stream_ptr, C.byref(cache._struct), k.data_ptr(), ldk, v.data_ptr(), ldv,
+    sess, stream, guard = launch_context(cache.device)
+    with guard:
+        check(lib.tfccb200_cache_append_f32(stream, cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv,
                                             ps, pl, pt, batch, width, k.shape[0], sess.status_ptr))
 
 
@@ -131,9 +133,9 @@ def read(cache: PagedCache, starts: torch.Tensor, lengths: torch.Tensor, table: 
     k, v = out
     ldk = _packed(k, "out[0]", rows, cols, cache.device)
     ldv = _packed(v, "out[1]", rows, cols, cache.device)
-    sess = get_session(cache.device)
-    with torch.cuda.device(cache.device):
-        check(lib.tfccb200_cache_read_f32(sess.stream_ptr, C.byref(cache._struct), k.data_ptr(), ldk, v.data_ptr(), ldv,
+    sess, stream, guard = launch_context(cache.device)
+    with guard:
+        check(lib.tfccb200_cache_read_f32(stream, cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv,
                                           ps, pl, pt, batch, width, rows, sess.status_ptr))
     return k, v
 
@@ -167,11 +169,11 @@ def attention(cache: PagedCache, q: torch.Tensor, starts: torch.Tensor, lengths:
     heads = cols // cache.dim
     if scale is None:
         scale = 1.0 / float(cache.dim) ** 0.5
-    sess = get_session(cache.device)
-    with torch.cuda.device(cache.device):
-        ws_ptr, ws_len = sess.workspace(lib.tfccb200_cache_attention_workspace(C.byref(cache._struct), batch, rows, heads,
-                                                                               max_new, max_length))
-        check(lib.tfccb200_cache_attention_f32(sess.stream_ptr, C.byref(cache._struct), q.data_ptr(), ldq, out.data_ptr(),
+    sess, stream, guard = launch_context(cache.device)
+    with guard:
+        ws_ptr, ws_len = sess.workspace_on(
+            lib.tfccb200_cache_attention_workspace(cache._ref, batch, rows, heads, max_new, max_length), stream)
+        check(lib.tfccb200_cache_attention_f32(stream, cache._ref, q.data_ptr(), ldq, out.data_ptr(),
                                                ldo, ps, pl, pt, batch, width, rows, heads, max_new, max_length,
                                                float(scale), 1 if causal else 0, ws_ptr, ws_len, sess.status_ptr))
     return out

@@ -13,7 +13,7 @@ import torch
 
 from . import exceptions
 from ._lib import ACTIVATIONS, PATHS, check, lib
-from .session import get_session
+from .session import get_session, launch_context
 
 _REDUCE = {torch.uint8: "tfccb200_reduce_sum_u8", torch.int8: "tfccb200_reduce_sum_s8",
            torch.int16: "tfccb200_reduce_sum_s16"}
@@ -269,6 +269,14 @@ def _rows(t, name, dtype):
         raise exceptions.NotImplementedError(f"{name}: implemented for {dtype}, got {t.dtype}")
     if not t.is_cuda:
         raise exceptions.InvalidArgumentError(f"{name} must be a CUDA tensor")
+    if t.dim() == 2:
+        rows, cols = t.shape
+        pitch, step = t.stride()
+        if rows == 1:
+            pitch = max(pitch, cols)  # the stride of a single row says nothing
+        if (cols != 1 and step != 1) or pitch < cols:
+            raise exceptions.InvalidArgumentError(f"{name}: rows must be contiguous and must not overlap")
+        return pitch, rows, cols
     shape, stride = t.shape, t.stride()
     cols = shape[-1]
     rows, pitch = shape[-2], stride[-2]
@@ -304,9 +312,9 @@ def quantize_tokens(a: torch.Tensor):
     shape = list(a.shape)
     codes = torch.empty(shape[:-1] + [wide], dtype=torch.int8, device=a.device)
     scales = torch.empty(shape[:-1], dtype=torch.float32, device=a.device)
-    sess = get_session(a.device)
-    with torch.cuda.device(a.device):
-        check(lib.tfccb200_quantize_tokens_f32(sess.stream_ptr, a.data_ptr(), pitch, rows, cols,
+    _, stream, guard = launch_context(a.device)
+    with guard:
+        check(lib.tfccb200_quantize_tokens_f32(stream, a.data_ptr(), pitch, rows, cols,
                                                codes.data_ptr(), wide, scales.data_ptr()))
     return codes[..., :cols], scales
 
@@ -343,9 +351,9 @@ def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     sb = _vector(b_scales, "b_scales", n, a.device)
     sbias = None if bias is None else _vector(bias, "bias", n, a.device)
     out = torch.empty(list(a.shape[:-1]) + [n], dtype=torch.float32, device=a.device)
-    sess = get_session(a.device)
-    with torch.cuda.device(a.device):
-        check(lib.tfccb200_qgemm_scaled_s8(sess.stream_ptr, a.data_ptr(), lda, sa, b.data_ptr(), ldb,
+    sess, stream, guard = launch_context(a.device)
+    with guard:
+        check(lib.tfccb200_qgemm_scaled_s8(stream, a.data_ptr(), lda, sa, b.data_ptr(), ldb,
                                            sb, sbias, out.data_ptr(), m, n, k,
                                            ACTIVATIONS[activation], PATHS[path], sess.status_ptr))
     return out
@@ -365,11 +373,11 @@ def linear(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch
         raise exceptions.InvalidArgumentError("unknown activation")
     sb = _vector(b_scales, "b_scales", n, x.device)
     sbias = None if bias is None else _vector(bias, "bias", n, x.device)
-    out = torch.empty(list(x.shape[:-1]) + [n], dtype=torch.float32, device=x.device)
-    sess = get_session(x.device)
-    with torch.cuda.device(x.device):
-        ws_ptr, ws_len = sess.workspace(lib.tfccb200_qlinear_workspace(m, k))
-        check(lib.tfccb200_qlinear_f32(sess.stream_ptr, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias,
+    out = torch.empty(x.shape[:-1] + (n,), dtype=torch.float32, device=x.device)
+    sess, stream, guard = launch_context(x.device)
+    with guard:
+        ws_ptr, ws_len = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k), stream)
+        check(lib.tfccb200_qlinear_f32(stream, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias,
                                        out.data_ptr(), m, n, k, ACTIVATIONS[activation], ws_ptr, ws_len,
                                        sess.status_ptr))
     return out

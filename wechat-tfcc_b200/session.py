@@ -33,6 +33,13 @@ class Session:
     def status_ptr(self) -> int:
         return self._status.data_ptr()
 
+    def workspace_on(self, nbytes: int, stream_ptr: int):
+        """:meth:`workspace` for a caller that already has the current stream's handle."""
+        ws = self._workspaces.get(stream_ptr)
+        if nbytes and ws is not None and ws.numel() >= nbytes:
+            return ws.data_ptr(), ws.numel()
+        return self.workspace(nbytes)
+
     def workspace(self, nbytes: int):
         """Scratch of at least ``nbytes`` for calls on the current stream (grown
         geometrically, reused by later calls on that stream).  A buffer that is outgrown is
@@ -60,6 +67,32 @@ class Session:
                 raise exceptions.InvalidArgumentError(
                     f"a cache operator met sequences or pages out of range (bits 0x{st:x})")
             raise exceptions.RuntimeError(-6, f"a kernel abandoned a bounded wait (bits 0x{st:x})")
+
+
+def launch_context(device):
+    """``(session, current stream's handle, guard)`` for a call on a tensor's device.  The launches of
+    one decode step take a few microseconds each, so this avoids what a call can do without: the guard
+    that makes ``device`` current is a no-op when it already is."""
+    index = device.index
+    table = getattr(_local, "sessions", None)
+    sess = table.get(index) if table is not None else None
+    if sess is None:
+        sess = get_session(device)
+    return sess, _raw_stream(index), _NO_GUARD if _current_device() == index else torch.cuda.device(device)
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def get_session(device) -> Session:
