@@ -6,15 +6,15 @@
 // with j over the cached tokens that token i sees: all of them, or (causal) those at positions up
 // to its own.  A row that sees nothing is 0.
 //
-// Arithmetic (both kernels).  A code is exact in fp16, so nothing is lost by handing K and V to
-// the tensor cores as fp16.  The fp32 operands are split into two fp16 terms, x = hi + lo with 11
-// bits each: q per row after scaling by a power of two, and the weights w_j = p_j vs_j, which carry
-// the value scales, after scaling by a power of two that bounds them.  Two products with fp32 sums
-// instead of one then give 22 bits, and the key scales are applied to the scores in fp32.  The softmax is
-// the one-pass form: running maximum and sum in fp32, sums rescaled when the maximum grows.
+// The weights w_j = p_j vs_j carry the value scales.  Codes are exact in fp16, and a weight is split into
+// two fp16 terms, w = hi + lo with 11 bits each, after scaling by a power of two that bounds the
+// weights; two products with fp32 sums then give 22 bits where one would give 11.  The softmax is
+// the one-pass form: a reference maximum and a sum in fp32, sums rescaled when a score exceeds the
+// reference by more than kLazy (in log2 units), which is rare after the first keys.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_attention.cuh"
 #include "internal.h"
@@ -28,11 +28,16 @@ namespace {
 // ---- few rows: memory-bound ----------------------------------------------------------------------
 //
 // Up to 8 (or 16) rows of a kv head against its whole cache: every code is used for a handful
-// of products, so what counts is streaming the cache.  A warp works alone: it brings 16 keys and their values
-// at a time through its own ring of cp.async stages (no CTA barrier in the loop) and multiplies with
-// mma.sync m16n8k16, whose operand fragments can be read straight from the rows as they lie
-// because the order of k is free: a lane's 16 bytes of a key row serve as its k slots of
-// successive steps.  With 8 rows the 16 rows of the instruction hold their hi and lo terms side by side.
+// of products, so what counts is streaming the cache and spending few instructions on a code.  A warp
+// works alone: it brings 16 keys and their values at a time through its own ring of cp.async stages (no
+// CTA barrier in the loop) and multiplies with mma.sync, whose fragments are read straight from
+// the rows as they lie because the order of k is free: a lane's 16 bytes of a key row serve as its k slots of
+// successive steps.
+//   Scores: q is a 24-bit integer per element (scaled by a power of two per row) in three balanced
+//   8-bit digits, and the codes are multiplied as they are, m16n8k32 in integers: exact sums and no conversion of
+//   K at all.  With 8 rows two digits fill the 16 rows of one product, the third a second one.
+//   Output: V becomes fp16 (1.5 instructions a code), weights as above; with 8 rows the 16 rows of
+//   m16n8k16 hold their hi and lo terms side by side.
 // Eight warps take the eight 16-key groups of a 128-key block and are added at the item's end.
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -43,7 +48,7 @@ struct FewLayout {
   static constexpr int kCodeBytes = 16 * DIM;               // codes of 16 keys (or values)
   static constexpr int kStageBytes = 2 * kCodeBytes + 128;  // + their scales
   static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
-  static constexpr int kFragBytes = (ROWS / 8) * (DIM / 16) * 32 * 16;
+  static constexpr int kFragBytes = (DIM / 32) * 32 * (ROWS == 8 ? 16 + 8 : 3 * 16);  // digits of q
   static constexpr int kSmall = kFragBytes + kFewWarps * kRingBytes;
   static constexpr int kSmem = kSmall + (kFewWarps * 2 * ROWS + kFewWarps) * 4;
   static_assert(ROWS * DIM * 4 <= kRingBytes, "a warp's sums reuse its ring");
@@ -59,6 +64,26 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// Four 24-bit integers -> three words of their balanced base-256 digits, lowest first.
+__device__ __forceinline__ void digits4(const int (&v)[4], uint32_t (&d)[3]) {
+  uint32_t x[4][3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d0 = static_cast<int8_t>(v[i]), r1 = (v[i] - d0) >> 8;
+    const int d1 = static_cast<int8_t>(r1), d2 = (r1 - d1) >> 8;
+    x[i][0] = d0 & 0xff; x[i][1] = d1 & 0xff; x[i][2] = d2 & 0xff;
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) d[k] = x[0][k] | (x[1][k] << 8) | (x[2][k] << 16) | (x[3][k] << 24);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
@@ -83,14 +108,15 @@ __device__ __forceinline__ unsigned value_chunk(unsigned r, unsigned c) {
   else return (r >> 1) * 128 + (((((r & 1u) << 2) + c) ^ (r & 6u)) << 4);
 }
 
-constexpr float kWeightTop = 16384.f;        // weights are scaled to at most 2^14: fp16 keeps 22 bits of
-                                             // them down to 2^-17 of the largest
+constexpr float kWeightTop = 1024.f;           // weights are scaled to at most 2^10, times 2^kLazy: fp16
+constexpr float kLazy = 5.f;                   // keeps 22 bits of them down to 2^-13 of the top
 constexpr float kValueFloor = 7.8886091e-31f;  // 2^-100
 
 template <int DIM, int ROWS>
 __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(const __grid_constant__ CacheAttention a) {
   using L = FewLayout<DIM, ROWS>;
-  constexpr int kSteps = DIM / 16;   // k-steps of a score
+  constexpr int kSteps = DIM / 32;   // k-steps of a score
+  constexpr int kVecs = DIM / 16;    // quads of a row that a lane holds
   constexpr int kTiles = DIM / 8;    // 8-wide column tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ ScheduleShared sched;
@@ -118,17 +144,20 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
     const int b = item.b;
 
     // ---- the warp's loads: 16 keys of block `blk` into stage `st` ----
-    auto load = [&](unsigned blk, int st) {
-      const int key0 = static_cast<int>(blk * kBlockKeys + warp * 16);
-      const int pos = key0 + static_cast<int>(lane & 15u);
-      const bool live = pos < length;
-      const int page = live ? page_of(a.c, b, pos) : -1;
+    // `slot`: place of key lane % 16 of the group in the scale arrays, ~0u for none.  It is looked up
+    // a step ahead, so that the page table's latency is not in the way.
+    auto look_up = [&](unsigned blk) {
+      const unsigned pos = blk * kBlockKeys + warp * 16 + (lane & 15u);
+      if (blk >= item.hi || static_cast<int>(pos) >= length) return ~0u;
+      const int page = page_of(a.c, b, pos);
+      return page < 0 ? ~0u : static_cast<unsigned>(cache_slot(a.c, page, head, pos));
+    };
+    auto load = [&](unsigned slot, int st) {
       const uint32_t dst = ring_addr + st * L::kStageBytes;
       {  // scales: lanes 0-15 of the keys, 16-31 of the values
         const uint32_t d = dst + 2 * L::kCodeBytes + lane * 4;
-        if (page >= 0) {
-          const size_t at = cache_slot(a.c, page, head, pos);
-          cp_async_4(d, (lane < 16 ? a.c.key_scales : a.c.value_scales) + at);
+        if (slot != ~0u) {
+          cp_async_4(d, (lane < 16 ? a.c.key_scales : a.c.value_scales) + slot);
         } else {  // a page that does not exist shows as NaN (a place behind the end is masked anyway)
           *reinterpret_cast<uint32_t*>(ring + (d - ring_addr)) = 0x7fffffffu;
         }
@@ -138,24 +167,31 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const unsigned r = (i * 32 + lane) / kChunks, c = lane % kChunks;
-        const int pg = __shfl_sync(0xffffffffu, page, r);
-        const size_t at = (pg >= 0 ? cache_slot(a.c, pg, head, key0 + r) : 0) * DIM + c * 16;
-        cp_async_16(dst + key_chunk<DIM>(r, c), a.c.keys + at, pg >= 0);
-        cp_async_16(dst + L::kCodeBytes + value_chunk<DIM>(r, c), a.c.values + at, pg >= 0);
+        const unsigned sl = __shfl_sync(0xffffffffu, slot, r);
+        const size_t at = (sl != ~0u ? static_cast<size_t>(sl) : 0) * DIM + c * 16;
+        cp_async_16(dst + key_chunk<DIM>(r, c), a.c.keys + at, sl != ~0u);
+        cp_async_16(dst + L::kCodeBytes + value_chunk<DIM>(r, c), a.c.values + at, sl != ~0u);
       }
     };
     auto has_keys = [&](unsigned blk) {  // warp-uniform
       return blk < item.hi && static_cast<int>(blk * kBlockKeys + warp * 16) < length;
     };
+    unsigned next_slot;
+    {
+      unsigned slot[L::kStages];
 #pragma unroll
-    for (int s = 0; s < L::kStages - 1; ++s) {
-      if (has_keys(item.lo + s)) load(item.lo + s, s);
-      cp_async_commit();
+      for (int s = 0; s < L::kStages; ++s) slot[s] = look_up(item.lo + s);
+#pragma unroll
+      for (int s = 0; s < L::kStages - 1; ++s) {
+        if (has_keys(item.lo + s)) load(slot[s], s);
+        cp_async_commit();
+      }
+      next_slot = slot[L::kStages - 1];
     }
 
-    // ---- query fragments: hi and lo terms of the rows, scaled by a power of two per row ----
-    // Lane (g, t) holds row g's (and, 16 rows, row g + 8's) values d = 64 [step >= 4] + 16 t +
-    // 4 (step & 3) + 0..3 as the k slots 2t, 2t+1, 2t+8, 2t+9 of k-step `step`.
+    // ---- digits of the rows of q, scaled by a power of two per row ----
+    // Lane (g, t) holds row g's (and, 16 rows, row g + 8's) values d = 64 [i >= 4] + 16 t + 4 (i & 3) + 0..3
+    // for i = 0 .. DIM / 16 - 1, and i = 2 s, 2 s + 1 are its k slots of step s.
     float row_scale[ROWS / 8];
     int sees[ROWS / 8];
 #pragma unroll
@@ -166,37 +202,44 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       sees[h] = !live ? 0 : (a.causal ? past + static_cast<int>(tok) + 1 : length);
       const float* src = a.q + a.ldq * (static_cast<size_t>(item.seq.first) + (live ? tok : 0)) +
                          (static_cast<size_t>(head) * a.group + (live ? r % a.group : 0)) * DIM;
-      float4 f[kSteps];
+      float4 f[kVecs];
       uint32_t m = 0;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        f[s] = live ? *reinterpret_cast<const float4*>(src + (s >> 2) * 64 + 16 * t + 4 * (s & 3))
+      for (int i = 0; i < kVecs; ++i) {
+        f[i] = live ? *reinterpret_cast<const float4*>(src + (i >> 2) * 64 + 16 * t + 4 * (i & 3))
                     : make_float4(0.f, 0.f, 0.f, 0.f);
-        f[s].x *= a.scale; f[s].y *= a.scale; f[s].z *= a.scale; f[s].w *= a.scale;
-        m = max(m, max(max(__float_as_uint(f[s].x) & 0x7fffffffu, __float_as_uint(f[s].y) & 0x7fffffffu),
-                       max(__float_as_uint(f[s].z) & 0x7fffffffu, __float_as_uint(f[s].w) & 0x7fffffffu)));
+        f[i].x *= a.scale; f[i].y *= a.scale; f[i].z *= a.scale; f[i].w *= a.scale;
+        m = max(m, max(max(__float_as_uint(f[i].x) & 0x7fffffffu, __float_as_uint(f[i].y) & 0x7fffffffu),
+                       max(__float_as_uint(f[i].z) & 0x7fffffffu, __float_as_uint(f[i].w) & 0x7fffffffu)));
       }
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      // 2^(10 - exponent): the row's largest value lands in [2^10, 2^11).  Zero and tiny rows (below
-      // 2^-100) take the bound of the range, a non-finite row 1 (it becomes NaN in any case).
+      // 2^(21 - exponent): the row's largest value lands in [2^21, 2^22), inside three balanced digits.  Zero and
+      // tiny rows (below 2^-100) take the bound of the range; a row with an infinity or a NaN is NaN.
       const int ex = static_cast<int>(m >> 23) - 127;
-      const int sh = ex == 128 ? 0 : 10 - max(ex, -100);
+      const int sh = ex == 128 ? 0 : 21 - max(ex, -100);
       const float up = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
-      row_scale[h] = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+      row_scale[h] = ex == 128 ? __uint_as_float(0x7fffffffu) : __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s % kFewWarps != static_cast<int>(warp) % kSteps) continue;
-        const float x = f[s].x * up, y = f[s].y * up, z = f[s].z * up, w = f[s].w * up;
-        const uint32_t h0 = pack_half2(x, y), h1 = pack_half2(z, w);
-        const uint32_t l0 = pack_rest(x, y, h0), l1 = pack_rest(z, w, h1);
+        uint32_t d[2][3];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 x = f[2 * s + e];
+          const int v[4] = {__float2int_rn(x.x * up), __float2int_rn(x.y * up), __float2int_rn(x.z * up), __float2int_rn(x.w * up)};
+          digits4(v, d[e]);
+        }
         if constexpr (ROWS == 8) {
-          frag[s * 32 + lane] = make_uint4(h0, l0, h1, l1);
+          frag[s * 32 + lane] = make_uint4(d[0][2], d[0][1], d[1][2], d[1][1]);
+          reinterpret_cast<uint2*>(frag + kSteps * 32)[s * 32 + lane] = make_uint2(d[0][0], d[1][0]);
         } else {
-          uint32_t* hi = reinterpret_cast<uint32_t*>(frag + s * 32 + lane);
-          uint32_t* lo = reinterpret_cast<uint32_t*>(frag + (kSteps + s) * 32 + lane);
-          hi[h] = h0; hi[2 + h] = h1;
-          lo[h] = l0; lo[2 + h] = l1;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(frag + (k * kSteps + s) * 32 + lane);
+            w[h] = d[0][k];
+            w[2 + h] = d[1][k];
+          }
         }
       }
     }
@@ -207,92 +250,117 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-    float top[ROWS / 8], sum[ROWS / 8], vref = kValueFloor;
+    float top[ROWS / 8], sum[ROWS / 8], vref = kValueFloor, vup = kWeightTop / kValueFloor;
 #pragma unroll
     for (int h = 0; h < ROWS / 8; ++h) top[h] = -INFINITY, sum[h] = 0.f;
 
     int st = 0;
-    for (unsigned blk = item.lo; blk < item.hi; ++blk) {
-      if (!has_keys(blk)) break;  // nor do later blocks have any for this warp
+    // keys below this are seen by every row of the item
+    const int all_see = a.causal ? past + static_cast<int>(item.tile * ROWS / a.group) + 1 : length;
+    // One group of 16 keys; kMask: with keys that not every row sees (compiled apart).
+    auto group16 = [&](unsigned blk, auto mask) {
+      constexpr bool kMask = decltype(mask)::value;
       cp_async_wait<L::kStages - 2>();
       __syncwarp();
       const uint8_t* stage = ring + st * L::kStageBytes;
       {
         const unsigned ahead = blk + L::kStages - 1;
-        if (has_keys(ahead)) load(ahead, st == 0 ? L::kStages - 1 : st - 1);
+        if (has_keys(ahead)) load(next_slot, st == 0 ? L::kStages - 1 : st - 1);
         cp_async_commit();
+        next_slot = look_up(ahead + 1);
       }
       if (++st == L::kStages) st = 0;
 
-      // scores of keys 0-7 and 8-15 of the group
-      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+      // scores of keys 0-7 and 8-15 of the group: [2 j + e] of a lane (g, t) are keys 2 t + e (+ 8 j)
+      float x[ROWS / 8][4];
+      {
+        int c[ROWS == 8 ? 2 : 3][2][4];
 #pragma unroll
-      for (int c = 0; c < DIM / 64; ++c) {
-        const uint4 ka = *reinterpret_cast<const uint4*>(stage + key_chunk<DIM>(g, c * 4 + t));
-        const uint4 kb = *reinterpret_cast<const uint4*>(stage + key_chunk<DIM>(g + 8, c * 4 + t));
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        for (int k = 0; k < (ROWS == 8 ? 2 : 3); ++k)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t ua = wa[w] ^ 0x80808080u, ub = wb[w] ^ 0x80808080u;
-          const uint32_t a0 = codes_low(ua), a1 = codes_high(ua), b0 = codes_low(ub), b1 = codes_high(ub);
-          const uint4 q = frag[(c * 4 + w) * 32 + lane];
-          mma_f16(s0, q, a0, a1);
-          mma_f16(s1, q, b0, b1);
-          if constexpr (ROWS == 16) {
-            const uint4 ql = frag[(kSteps + c * 4 + w) * 32 + lane];
-            mma_f16(s0, ql, a0, a1);
-            mma_f16(s1, ql, b0, b1);
+          for (int i = 0; i < 4; ++i) c[k][0][i] = c[k][1][i] = 0;
+#pragma unroll
+        for (int q = 0; q < DIM / 64; ++q) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(stage + key_chunk<DIM>(g, q * 4 + t));
+          const uint4 kb = *reinterpret_cast<const uint4*>(stage + key_chunk<DIM>(g + 8, q * 4 + t));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int s = 2 * q + e;
+            const uint32_t a0 = e ? ka.z : ka.x, a1 = e ? ka.w : ka.y, b0 = e ? kb.z : kb.x, b1 = e ? kb.w : kb.y;
+            if constexpr (ROWS == 8) {
+              const uint4 f = frag[s * 32 + lane];
+              const uint2 l = reinterpret_cast<const uint2*>(frag + kSteps * 32)[s * 32 + lane];
+              const uint4 fl = make_uint4(l.x, 0u, l.y, 0u);
+              mma_s8(c[0][0], f, a0, a1);
+              mma_s8(c[0][1], f, b0, b1);
+              mma_s8(c[1][0], fl, a0, a1);
+              mma_s8(c[1][1], fl, b0, b1);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 3; ++k) {
+                const uint4 f = frag[(k * kSteps + s) * 32 + lane];
+                mma_s8(c[k][0], f, a0, a1);
+                mma_s8(c[k][1], f, b0, b1);
+              }
+            }
           }
         }
+        // high digit * 2^16 + (middle * 2^8 + low): the bracket stays below 2^30
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (ROWS == 8) {
+              x[0][2 * j + e] = fmaf(static_cast<float>(c[0][j][e]), 65536.f,
+                                     static_cast<float>(c[0][j][2 + e] * 256 + c[1][j][e]));
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                x[h][2 * j + e] = fmaf(static_cast<float>(c[2][j][2 * h + e]), 65536.f,
+                                       static_cast<float>(c[1][j][2 * h + e] * 256 + c[0][j][2 * h + e]));
+            }
+          }
       }
-      // lane (g, t): keys 2t, 2t+1, 2t+8, 2t+9 of rows g (and g + 8)
       const float* ks = reinterpret_cast<const float*>(stage + 2 * L::kCodeBytes);
       const float2 ka = *reinterpret_cast<const float2*>(ks + 2 * t), kb = *reinterpret_cast<const float2*>(ks + 2 * t + 8);
       const float2 va = *reinterpret_cast<const float2*>(ks + 16 + 2 * t), vb = *reinterpret_cast<const float2*>(ks + 24 + 2 * t);
       const int key0 = static_cast<int>(blk * kBlockKeys + warp * 16 + 2 * t);
-      const float kscale[4] = {ka.x, ka.y, kb.x, kb.y}, vscale[4] = {va.x, va.y, vb.x, vb.y};
-      float x[ROWS / 8][4];
-      if constexpr (ROWS == 8) {
-        x[0][0] = s0[0] + s0[2]; x[0][1] = s0[1] + s0[3]; x[0][2] = s1[0] + s1[2]; x[0][3] = s1[1] + s1[3];
-      } else {
-        x[0][0] = s0[0]; x[0][1] = s0[1]; x[0][2] = s1[0]; x[0][3] = s1[1];
-        x[1][0] = s0[2]; x[1][1] = s0[3]; x[1][2] = s1[2]; x[1][3] = s1[3];
-      }
+      const float kscale[4] = {ka.x, ka.y, kb.x, kb.y};
+      float vscale[4] = {va.x, va.y, vb.x, vb.y};
       bool grows = false;
-      float next_top[ROWS / 8];
 #pragma unroll
       for (int h = 0; h < ROWS / 8; ++h) {
+        const float limit = top[h] + kLazy;  // -inf before the first key
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = key0 + (j & 1) + (j >> 1) * 8;
-          x[h][j] = key < sees[h] ? x[h][j] * (kscale[j] * row_scale[h]) : -INFINITY;
+          x[h][j] *= kscale[j] * row_scale[h];
+          if constexpr (kMask) x[h][j] = key0 + (j & 1) + (j >> 1) * 8 < sees[h] ? x[h][j] : -INFINITY;
+          grows |= x[h][j] > limit;
         }
-        float m = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        next_top[h] = fmaxf(top[h], m);
-        grows |= next_top[h] > top[h];
       }
-      // largest value scale of the group, rounded up to a power of two
-      float vmax = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int key = key0 + (j & 1) + (j >> 1) * 8;
-        if (key < length) vmax = fmaxf(vmax, fabsf(vscale[j]));
+        if constexpr (kMask) vscale[j] = key0 + (j & 1) + (j >> 1) * 8 < length ? vscale[j] : 0.f;
+        grows |= vscale[j] > vref;
       }
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-      grows |= vmax > vref;
       if (__any_sync(0xffffffffu, grows)) {
-        float vnext = vref;
+        float vmax = fmaxf(fmaxf(vscale[0], vscale[1]), fmaxf(vscale[2], vscale[3]));
+        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
+        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+        float vnext = vref;  // largest value scale so far, rounded up to a power of two
         if (vmax > vref) vnext = __uint_as_float(min((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
         const float vf = vref / vnext;
         vref = vnext;
+        vup = kWeightTop / vref;
 #pragma unroll
         for (int h = 0; h < ROWS / 8; ++h) {
-          const float f = exp2_fast(top[h] - (next_top[h] == -INFINITY ? 0.f : next_top[h]));
+          float m = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const float next = m > top[h] + kLazy ? m : top[h];
+          const float f = exp2_fast(top[h] - (next == -INFINITY ? 0.f : next));
           sum[h] *= f;
-          top[h] = next_top[h];
+          top[h] = next;
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) {
             o[i][2 * h] *= f * vf;
@@ -304,18 +372,20 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
           }
         }
       }
-      const float vup = kWeightTop / vref;
       uint32_t hi[ROWS / 8][2], lo[ROWS / 8][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vscale[j] *= vup;
 #pragma unroll
       for (int h = 0; h < ROWS / 8; ++h) {
         const float base = top[h] == -INFINITY ? 0.f : top[h];
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = key0 + (j & 1) + (j >> 1) * 8;
           const float p = exp2_fast(x[h][j] - base);
           sum[h] += p;
-          w[j] = key < sees[h] ? p * (vscale[j] * vup) : 0.f;  // (0 * NaN behind the end would be NaN)
+          w[j] = p * vscale[j];
+          if constexpr (kMask)  // (0 * NaN)
+            w[j] = key0 + (j & 1) + (j >> 1) * 8 < sees[h] ? w[j] : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -360,6 +430,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
         }
       }
       __syncwarp();  // the stage may be overwritten
+    };
+    for (unsigned blk = item.lo; blk < item.hi; ++blk) {
+      if (!has_keys(blk)) break;  // nor do later blocks have any for this warp
+      if (static_cast<int>(blk * kBlockKeys + warp * 16 + 16) > all_see) group16(blk, std::true_type());
+      else group16(blk, std::false_type());
     }
     cp_async_wait<0>();
 

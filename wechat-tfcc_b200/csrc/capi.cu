@@ -871,7 +871,9 @@ int fill_cache(CacheArgs& a, void* stream, const tfccb200_cache* c, const int32_
     return TFCCB200_EALIGN;
   // page numbers and positions are int32
   if (c->pages > 0x7fffffffu || rows > 0x7fffffffu || c->kv_heads > 65535u || batch > (1u << 24) ||
-      static_cast<unsigned long long>(table_width) * c->page_size > 0x7fffff00ull)
+      static_cast<unsigned long long>(table_width) * c->page_size > 0x7fffff00ull ||
+      // (the kernels count places in 32 bits: 137 GB of keys at dim 64)
+      static_cast<unsigned long long>(c->pages) * c->kv_heads * c->page_size > 0x7fffffffull)
     return TFCCB200_EOVERFLOW;
   a.stream = static_cast<cudaStream_t>(stream);
   a.keys = c->keys; a.key_scales = c->key_scales;
