@@ -132,8 +132,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
 
   unsigned long long mine;
   const unsigned long long units = all_units<ROWS, kFewThreads>(a, &sched, &mine);
-  const unsigned long long u0 = range_begin(units, a.grid, blockIdx.x);
-  const unsigned long long u1 = range_begin(units, a.grid, blockIdx.x + 1);
+  const unsigned busy = busy_ctas(units, a.grid);
+  const bool mine_any = blockIdx.x < busy;
+  const unsigned long long u0 = mine_any ? range_begin(units, busy, blockIdx.x) : 0;
+  const unsigned long long u1 = mine_any ? range_begin(units, busy, blockIdx.x + 1) : 0;
   if (u0 == u1) return;
   find_unit<ROWS, kFewThreads>(a, u0, mine, &sched);
 
@@ -511,7 +513,7 @@ constexpr unsigned kFewCtasPerSm = 2;
 // Largest number of units a launch of these bounds can have.
 unsigned long long few_units_bound(const CacheAttentionArgs& a) {
   return static_cast<unsigned long long>(a.cache.batch) * a.cache.kv_heads *
-         ((a.max_length + kBlockKeys - 1) / kBlockKeys);
+         ((a.max_length + kBlockKeys - 1) / kBlockKeys + kLeadUnits);
 }
 
 template <int DIM, int ROWS>

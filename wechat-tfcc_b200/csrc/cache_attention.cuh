@@ -72,8 +72,8 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t u) { return unbias(__byt
 // ---- the pieces of cut items ---------------------------------------------------------------------
 //
 // CTA c looks at the boundary between ranges c and c + 1 (those of the attention kernel).  If that is the
-// first boundary inside an item, it adds the item's pieces in key order; blockIdx.y shares out
-// the item's elements.
+// first boundary among the blocks of an item, it adds the item's pieces, which are those of ranges
+// c, c + 1, ... up to the item's end, in key order; blockIdx.y shares out the item's elements.
 template <int DIM, int ROWS>
 static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const __grid_constant__ CacheAttention a) {
   __shared__ ScheduleShared sched;
@@ -81,39 +81,59 @@ static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const
   pdl_wait();
   unsigned long long mine;
   const unsigned long long units = all_units<ROWS, 256>(a, &sched, &mine);
-  const unsigned c = blockIdx.x + 1;
-  const unsigned long long at = range_begin(units, a.grid, c);
-  if (at >= units) return;
+  const unsigned busy = busy_ctas(units, a.grid), c = blockIdx.x;
+  if (c + 1 >= busy) return;
+  const unsigned long long at = range_begin(units, busy, c + 1);
   find_unit<ROWS, 256>(a, at, mine, &sched);
-  const ItemWalk<ROWS> item(a, 1, &sched);
-  if (item.lo == 0) return;  // the boundary lies between two items
-  const unsigned long long begin = at - item.lo, end = begin + item.blocks;
-  if (range_begin(units, a.grid, c - 1) > begin) return;  // not the item's first
-  const unsigned rows = static_cast<unsigned>(item.seq.count) * a.group;
+  // the item that unit `at` lies in, and its place there
+  const int b = sched.seq;
+  const DeviceSequence seq = load_sequence(a.c, b);
+  const unsigned per_head = head_units<ROWS>(a, seq);
+  const unsigned head = static_cast<unsigned>(sched.rem / per_head);
+  unsigned place = static_cast<unsigned>(sched.rem % per_head), tile = 0, blocks;
+  while (true) {
+    blocks = tile_blocks<ROWS>(a, seq, tile);
+    if (place < blocks + kLeadUnits) break;
+    place -= blocks + kLeadUnits;
+    ++tile;
+  }
+  if (place <= kLeadUnits) return;  // nothing of the item lies before the boundary
+  const unsigned long long first = at - place + kLeadUnits, end = at - place + kLeadUnits + blocks;  // its blocks' units
+  if (range_begin(units, busy, c) > first) return;  // not the first boundary among them
+  // the range that holds the item's last unit
+  unsigned last = static_cast<unsigned>(min(static_cast<unsigned long long>(busy - 1), (end - 1) * busy / units));
+  while (range_begin(units, busy, last) > end - 1) --last;
+  while (last + 1 < busy && range_begin(units, busy, last + 1) <= end - 1) ++last;
+  const unsigned rows = static_cast<unsigned>(seq.count) * a.group;
+  constexpr size_t kPitch = 2 * piece_floats<ROWS, DIM>();  // from one range's slot to the next one's
+  const float* const p1 = piece<ROWS, DIM>(a, c, true);     // the piece that begins with the item
+  const float* const p0 = piece<ROWS, DIM>(a, c, false) + kPitch;
+  const unsigned more = last - c;  // pieces after the first
   for (unsigned e = (blockIdx.y * 256 + threadIdx.x) * 4; e < ROWS * DIM; e += gridDim.y * 1024) {
-    const unsigned r = e / DIM, d = e % DIM, row = item.tile * ROWS + r;
+    const unsigned r = e / DIM, d = e % DIM, row = tile * ROWS + r;
     if (row >= rows) continue;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    unsigned long long from = begin;
-    for (unsigned k = c - 1; from < end; ++k) {
-      const unsigned long long to = range_begin(units, a.grid, k + 1);
-      if (to <= from) continue;  // an empty range, or the part of range c - 1 before the item
-      const float* p = piece<ROWS, DIM>(a, k, k == c - 1);
-      const float pm = __ldg(p + r), pl = __ldg(p + ROWS + r);
+    const float m1 = __ldg(p1 + r);
+    float m = m1;
+#pragma unroll 8
+    for (unsigned k = 0; k < more; ++k) m = fmaxf(m, __ldg(p0 + k * kPitch + r));
+    const float base = m == -INFINITY ? 0.f : m;
+    float f = exp2_fast(m1 - base);
+    float l = f * __ldg(p1 + ROWS + r);
+    const float4 y1 = __ldg(reinterpret_cast<const float4*>(p1 + 2 * ROWS + e));
+    float4 acc = make_float4(f * y1.x, f * y1.y, f * y1.z, f * y1.w);
+#pragma unroll 8
+    for (unsigned k = 0; k < more; ++k) {
+      const float* p = p0 + k * kPitch;
       const float4 y = __ldg(reinterpret_cast<const float4*>(p + 2 * ROWS + e));
-      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
-      const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
-      m = next;
-      l = f * l + g * pl;
-      acc.x = f * acc.x + g * y.x; acc.y = f * acc.y + g * y.y;
-      acc.z = f * acc.z + g * y.z; acc.w = f * acc.w + g * y.w;
-      from = to;
+      f = exp2_fast(__ldg(p + r) - base);
+      l = fmaf(f, __ldg(p + ROWS + r), l);
+      acc.x = fmaf(f, y.x, acc.x); acc.y = fmaf(f, y.y, acc.y);
+      acc.z = fmaf(f, y.z, acc.z); acc.w = fmaf(f, y.w, acc.w);
     }
     const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     const unsigned tok = row / a.group;
-    float* dst = a.out + a.ldo * (static_cast<size_t>(item.seq.first) + tok) +
-                 (static_cast<size_t>(item.head) * a.group + row % a.group) * DIM + d;
+    float* dst = a.out + a.ldo * (static_cast<size_t>(seq.first) + tok) +
+                 (static_cast<size_t>(head) * a.group + row % a.group) * DIM + d;
     *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }

@@ -155,8 +155,10 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
 
   unsigned long long mine;
   const unsigned long long units = all_units<kManyRows, kThreads>(a, sched, &mine);
-  const unsigned long long u0 = range_begin(units, a.grid, blockIdx.x);
-  const unsigned long long u1 = range_begin(units, a.grid, blockIdx.x + 1);
+  const unsigned busy = busy_ctas(units, a.grid);
+  const bool mine_any = blockIdx.x < busy;
+  const unsigned long long u0 = mine_any ? range_begin(units, busy, blockIdx.x) : 0;
+  const unsigned long long u1 = mine_any ? range_begin(units, busy, blockIdx.x + 1) : 0;
   if (u0 < u1) find_unit<kManyRows, kThreads>(a, u0, mine, sched);
 
   // Hands every item to `body`; the stage is released when body has returned (and has therefore
@@ -612,7 +614,7 @@ int launch_many(const CacheAttentionArgs& args, CacheAttention a, int sm_count) 
   // for its ragged end) times the blocks of the longest
   const unsigned long long rows = static_cast<unsigned long long>(args.cache.rows) * a.group;
   const unsigned long long bound = (rows / kManyRows + args.cache.batch) * args.cache.kv_heads *
-                                   ((args.max_length + kBlockKeys - 1) / kBlockKeys);
+                                   ((args.max_length + kBlockKeys - 1) / kBlockKeys + kLeadUnits);
   a.grid = static_cast<unsigned>(bound < static_cast<unsigned long long>(sm_count) ? bound : sm_count);
   cudaError_t e = launch_after_previous(cache_attention_many_kernel<DIM>, dim3(a.grid), dim3(kThreads), L::kSmem,
                                         args.cache.stream, a, kDefaultTimeoutNs);

@@ -4,8 +4,10 @@
 // is new token r / group, query head r % group of the head's group), and its units are the blocks
 // of kBlockKeys cached tokens that the tile's last row sees.  Lengths are device data and differ, so no
 // grid the host could choose would be even: instead the units of all items are laid end to
-// end (sequence, head, tile, block) and every CTA takes an equal range of them.  A range may begin
-// and end inside an item.  Items that lie whole in one range are finished there; the pieces of a
+// end (sequence, head, tile, block), each item led by kLeadUnits that stand for what beginning and
+// ending an item costs, and every CTA takes an equal range.  (Without the lead a CTA that
+// drew eight short sequences took 85 us where the others took 60.)  A range may begin and end inside an
+// item.  Items that lie whole in one range are finished there; the pieces of a
 // cut one go to scratch as unnormalised sums with their maximum, and the merge kernel adds
 // them in key order.  Cuts depend on lengths and grid alone, so results repeat bit by bit.
 #pragma once
@@ -15,6 +17,7 @@
 namespace tfccb200 {
 
 constexpr unsigned kBlockKeys = 128;
+constexpr unsigned kLeadUnits = 2;
 // Sequences with up to this many rows per kv head go to the few-rows kernel.
 constexpr unsigned kFewRows = 16;
 
@@ -53,7 +56,7 @@ __device__ __forceinline__ unsigned sequence_tiles(const CacheAttention& a, cons
 template <int kRows>
 __device__ __forceinline__ unsigned head_units(const CacheAttention& a, const DeviceSequence& s) {
   const unsigned tiles = sequence_tiles<kRows>(a, s);
-  unsigned n = 0;
+  unsigned n = tiles * kLeadUnits;
   for (unsigned t = 0; t < tiles; ++t) n += tile_blocks<kRows>(a, s, t);
   return n;
 }
@@ -129,29 +132,35 @@ __device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long
   __syncthreads();
 }
 
-__device__ __forceinline__ unsigned long long range_begin(unsigned long long units, unsigned grid, unsigned cta) {
-  return units / grid * cta + units % grid * cta / grid;
+// CTAs that get a range: as many as there are units at most, so that no range is empty.
+__device__ __forceinline__ unsigned busy_ctas(unsigned long long units, unsigned grid) {
+  return units < grid ? static_cast<unsigned>(units) : grid;
+}
+__device__ __forceinline__ unsigned long long range_begin(unsigned long long units, unsigned busy, unsigned cta) {
+  return units / busy * cta + units % busy * cta / busy;
 }
 
-// Walks the items of a range of units.
+// Walks the items of a range of units; those of which the range holds no block are passed over.
 template <int kRows>
 struct ItemWalk {
   const CacheAttention& a;
   unsigned long long left;  // units still to come, this item's included
-  unsigned long long rem;   // this item's first unit within the sequence
+  unsigned long long rem;   // the range's first unit of this item within the sequence
   int b;
   DeviceSequence seq;
   unsigned per_head, head, tile, blocks;  // `blocks`: all of the item's
   unsigned lo, hi;                        // this range's blocks of it
+  unsigned taken;                         // this range's units of it
 
   __device__ ItemWalk(const CacheAttention& a_, unsigned long long units, const ScheduleShared* sh)
-      : a(a_), left(units), rem(0), b(0), per_head(0), head(0), tile(0), blocks(0), lo(0), hi(0) {
+      : a(a_), left(units), rem(0), b(0), per_head(0), head(0), tile(0), blocks(0), lo(0), hi(0), taken(0) {
     if (left == 0) return;
     b = sh->seq;
     rem = sh->rem;
     seq = load_sequence(a.c, b);
     per_head = head_units<kRows>(a, seq);
     place();
+    if (lo == hi) next();
   }
   __device__ void place() {
     head = static_cast<unsigned>(rem / per_head);
@@ -159,29 +168,32 @@ struct ItemWalk {
     tile = 0;
     while (true) {
       blocks = tile_blocks<kRows>(a, seq, tile);
-      if (at < blocks) break;
-      at -= blocks;
+      if (at < blocks + kLeadUnits) break;
+      at -= blocks + kLeadUnits;
       ++tile;
     }
-    lo = at;
-    hi = static_cast<unsigned>(min(static_cast<unsigned long long>(blocks), at + left));
+    const unsigned end = static_cast<unsigned>(min(static_cast<unsigned long long>(blocks + kLeadUnits), at + left));
+    taken = end - at;
+    lo = at < kLeadUnits ? 0 : at - kLeadUnits;
+    hi = end < kLeadUnits ? 0 : end - kLeadUnits;
   }
   __device__ bool done() const { return left == 0; }
   __device__ bool whole() const { return lo == 0 && hi == blocks; }
   __device__ void next() {
-    const unsigned n = hi - lo;
-    left -= n;
-    rem += n;
-    if (left == 0) return;
-    while (rem >= static_cast<unsigned long long>(per_head) * a.c.kv_heads) {
-      rem = 0;
-      do {
-        ++b;
-        seq = load_sequence(a.c, b);
-        per_head = head_units<kRows>(a, seq);
-      } while (per_head == 0);  // units are left, so a sequence that has some follows
-    }
-    place();
+    do {
+      left -= taken;
+      rem += taken;
+      if (left == 0) return;
+      while (rem >= static_cast<unsigned long long>(per_head) * a.c.kv_heads) {
+        rem = 0;
+        do {
+          ++b;
+          seq = load_sequence(a.c, b);
+          per_head = head_units<kRows>(a, seq);
+        } while (per_head == 0);  // units are left, so a sequence that has some follows
+      }
+      place();
+    } while (lo == hi);
   }
 };
 
