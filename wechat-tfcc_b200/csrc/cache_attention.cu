@@ -130,16 +130,24 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
   float* red_l = red_m + kFewWarps * ROWS;
   float* red_v = red_l + kFewWarps * ROWS;  // [warp]
 
-  unsigned long long mine;
+  ThreadSequence mine;
   const unsigned long long units = all_units<ROWS, kFewThreads>(a, &sched, &mine);
   const unsigned busy = busy_ctas(units, a.grid);
   const bool mine_any = blockIdx.x < busy;
   const unsigned long long u0 = mine_any ? range_begin(units, busy, blockIdx.x) : 0;
   const unsigned long long u1 = mine_any ? range_begin(units, busy, blockIdx.x + 1) : 0;
-  if (u0 == u1) return;
+  if (u0 == u1) {
+    if (a.scratch && tid == 0) write_note<ROWS>(a, blockIdx.x, busy, units, u1, nullptr);
+    return;
+  }
   find_unit<ROWS, kFewThreads>(a, u0, mine, &sched);
 
+  bool noted = false;
   for (ItemWalk<ROWS> item(a, u1 - u0, &sched); !item.done(); item.next()) {
+    if (a.scratch && item.taken == item.left) {  // the range's last
+      if (tid == 0) write_note<ROWS>(a, blockIdx.x, busy, units, u1, &item);
+      noted = true;
+    }
     const unsigned rows = static_cast<unsigned>(item.seq.count) * a.group;
     const int length = item.seq.length, past = length - item.seq.count;
     const unsigned head = item.head;
@@ -166,6 +174,23 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       }
       constexpr int kChunks = DIM / 16;  // 16-byte chunks of a row
       constexpr int kPer = 16 * kChunks / 32;
+      if (a.c.page_shift >= 4) {
+        // the 16 places follow one another in one page: two addresses, the rest are constant steps
+        const unsigned r0 = lane / kChunks, c = lane % kChunks;
+        const unsigned sl = __shfl_sync(0xffffffffu, slot, 0);  // (a group is loaded when its first key exists)
+        const unsigned n = __popc(__ballot_sync(0xffffffffu, slot != ~0u) & 0xffffu);
+        const size_t at = static_cast<size_t>(n ? sl + r0 : 0u) * DIM + c * 16;
+        const int8_t* const k = a.c.keys + at;
+        const int8_t* const v = a.c.values + at;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const unsigned r = i * (32 / kChunks) + r0;
+          const bool in = r < n;
+          cp_async_16(dst + key_chunk<DIM>(r, c), in ? k + i * (32 / kChunks) * DIM : a.c.keys, in);
+          cp_async_16(dst + L::kCodeBytes + value_chunk<DIM>(r, c), in ? v + i * (32 / kChunks) * DIM : a.c.values, in);
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const unsigned r = (i * 32 + lane) / kChunks, c = lane % kChunks;
@@ -504,6 +529,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
     }
     __syncthreads();  // rings, fragments and maxima are free for the next item
   }
+  if (a.scratch && !noted && tid == 0) write_note<ROWS>(a, blockIdx.x, busy, units, u1, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -532,7 +558,7 @@ int launch_few(const CacheAttentionArgs& args, CacheAttention a, int sm_count) {
   if (e != cudaSuccess) return static_cast<int>(e);
   count_launch();
   if (cut && a.grid > 1) {
-    e = launch_after_previous(cache_attention_merge_kernel<DIM, ROWS>, dim3(a.grid - 1), dim3(256), 0,
+    e = launch_after_previous(cache_attention_merge_kernel<DIM, ROWS>, dim3(a.grid), dim3(256), 0,
                               args.cache.stream, a);
     if (e != cudaSuccess) return static_cast<int>(e);
     count_launch();
@@ -552,10 +578,10 @@ size_t cache_attention_workspace(const CacheAttentionArgs& a) {
   const size_t sms = di ? di->sm_count : 148;
   if (a.max_length <= kBlockKeys) return 0;  // one block per item: nothing is cut
   const size_t row = (a.cache.dim + 2) * sizeof(float);
-  const size_t few = 2 * kFewCtasPerSm * sms * few_rows_of(a) * row;
+  const size_t few = kNotesBytes + 2 * kFewCtasPerSm * sms * few_rows_of(a) * row;
   const bool many = static_cast<unsigned long long>(a.max_new) * (a.heads / a.cache.kv_heads) > kFewRows;
   // the two kernels run one after the other and share it
-  return many ? std::max(few, 2 * sms * kManyRows * row) : few;
+  return many ? std::max(few, kNotesBytes + 2 * sms * kManyRows * row) : few;
 }
 
 int cache_attention(const CacheAttentionArgs& args) {
@@ -571,7 +597,7 @@ int cache_attention(const CacheAttentionArgs& args) {
   if (args.max_length < a.c.max_length) a.c.max_length = args.max_length;
   a.causal = args.causal;
   a.scale = args.scale * 1.4426950408889634f;
-  a.scratch = static_cast<float*>(args.workspace);
+  a.scratch = args.max_length > kBlockKeys ? static_cast<float*>(args.workspace) : nullptr;
   const bool wide = args.cache.dim == 128;
   int st = TFCCB200_OK;
   if (a.group <= kFewRows) {

@@ -71,47 +71,22 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t u) { return unbias(__byt
 
 // ---- the pieces of cut items ---------------------------------------------------------------------
 //
-// CTA c looks at the boundary between ranges c and c + 1 (those of the attention kernel).  If that is the
-// first boundary among the blocks of an item, it adds the item's pieces, which are those of ranges
-// c, c + 1, ... up to the item's end, in key order; blockIdx.y shares out the item's elements.
+// One CTA (or several, blockIdx.y sharing out the elements) per range of the attention kernel that began an item
+// without ending it: the item's pieces are added in key order.
 template <int DIM, int ROWS>
 static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const __grid_constant__ CacheAttention a) {
-  __shared__ ScheduleShared sched;
   pdl_release();
   pdl_wait();
-  unsigned long long mine;
-  const unsigned long long units = all_units<ROWS, 256>(a, &sched, &mine);
-  const unsigned busy = busy_ctas(units, a.grid), c = blockIdx.x;
-  if (c + 1 >= busy) return;
-  const unsigned long long at = range_begin(units, busy, c + 1);
-  find_unit<ROWS, 256>(a, at, mine, &sched);
-  // the item that unit `at` lies in, and its place there
-  const int b = sched.seq;
-  const DeviceSequence seq = load_sequence(a.c, b);
-  const unsigned per_head = head_units<ROWS>(a, seq);
-  const unsigned head = static_cast<unsigned>(sched.rem / per_head);
-  unsigned place = static_cast<unsigned>(sched.rem % per_head), tile = 0, blocks;
-  while (true) {
-    blocks = tile_blocks<ROWS>(a, seq, tile);
-    if (place < blocks + kLeadUnits) break;
-    place -= blocks + kLeadUnits;
-    ++tile;
-  }
-  if (place <= kLeadUnits) return;  // nothing of the item lies before the boundary
-  const unsigned long long first = at - place + kLeadUnits, end = at - place + kLeadUnits + blocks;  // its blocks' units
-  if (range_begin(units, busy, c) > first) return;  // not the first boundary among them
-  // the range that holds the item's last unit
-  unsigned last = static_cast<unsigned>(min(static_cast<unsigned long long>(busy - 1), (end - 1) * busy / units));
-  while (range_begin(units, busy, last) > end - 1) --last;
-  while (last + 1 < busy && range_begin(units, busy, last + 1) <= end - 1) ++last;
-  const unsigned rows = static_cast<unsigned>(seq.count) * a.group;
+  const unsigned c = blockIdx.x;
+  const PieceNote note = *piece_note(a, c);
+  const unsigned more = note.ranges;  // pieces after the first
+  if (more == 0) return;
   constexpr size_t kPitch = 2 * piece_floats<ROWS, DIM>();  // from one range's slot to the next one's
   const float* const p1 = piece<ROWS, DIM>(a, c, true);     // the piece that begins with the item
   const float* const p0 = piece<ROWS, DIM>(a, c, false) + kPitch;
-  const unsigned more = last - c;  // pieces after the first
   for (unsigned e = (blockIdx.y * 256 + threadIdx.x) * 4; e < ROWS * DIM; e += gridDim.y * 1024) {
-    const unsigned r = e / DIM, d = e % DIM, row = tile * ROWS + r;
-    if (row >= rows) continue;
+    const unsigned r = e / DIM, d = e % DIM, row = note.tile * ROWS + r;
+    if (row >= note.rows) continue;
     const float m1 = __ldg(p1 + r);
     float m = m1;
 #pragma unroll 8
@@ -132,8 +107,8 @@ static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const
     }
     const float inv = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
     const unsigned tok = row / a.group;
-    float* dst = a.out + a.ldo * (static_cast<size_t>(seq.first) + tok) +
-                 (static_cast<size_t>(head) * a.group + row % a.group) * DIM + d;
+    float* dst = a.out + a.ldo * (static_cast<size_t>(note.first) + tok) +
+                 (static_cast<size_t>(note.head) * a.group + row % a.group) * DIM + d;
     *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }

@@ -153,7 +153,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
   const uint32_t tmem = misc[0];
   pdl_wait();
 
-  unsigned long long mine;
+  ThreadSequence mine;
   const unsigned long long units = all_units<kManyRows, kThreads>(a, sched, &mine);
   const unsigned busy = busy_ctas(units, a.grid);
   const bool mine_any = blockIdx.x < busy;
@@ -296,8 +296,12 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         ++n;
         return true;
       };
-      bool live = true;
+      bool live = true, noted = false;
       for (ItemWalk<kManyRows> w(a, u1 - u0, sched); live && !w.done(); w.next()) {
+        if (a.scratch && w.taken == w.left) {  // the range's last
+          if (lane == 0) write_note<kManyRows>(a, blockIdx.x, busy, units, u1, &w);
+          noted = true;
+        }
         Item it;
         it.first = w.seq.first; it.count = w.seq.count; it.length = w.seq.length; it.b = w.b;
         it.head = w.head; it.tile = w.tile; it.lo = w.lo; it.hi = w.hi;
@@ -305,6 +309,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         it.rows = static_cast<unsigned>(w.seq.count) * a.group;
         live = put(it);
       }
+      if (a.scratch && !noted && lane == 0) write_note<kManyRows>(a, blockIdx.x, busy, units, u1, nullptr);
       Item end = {};
       if (live) put(end);
     }
@@ -621,7 +626,7 @@ int launch_many(const CacheAttentionArgs& args, CacheAttention a, int sm_count) 
   if (e != cudaSuccess) return static_cast<int>(e);
   count_launch();
   if (args.max_length > kBlockKeys && a.grid > 1) {
-    e = launch_after_previous(cache_attention_merge_kernel<DIM, kManyRows>, dim3(a.grid - 1, 4), dim3(256), 0,
+    e = launch_after_previous(cache_attention_merge_kernel<DIM, kManyRows>, dim3(a.grid, 4), dim3(256), 0,
                               args.cache.stream, a);
     if (e != cudaSuccess) return static_cast<int>(e);
     count_launch();

@@ -62,9 +62,11 @@ __device__ __forceinline__ unsigned head_units(const CacheAttention& a, const De
 }
 
 struct ScheduleShared {
-  unsigned long long sums[33];
-  unsigned long long rem;
-  int seq;
+  unsigned long long sums[32];
+  unsigned long long rem;  // find_unit: place within the sequence,
+  int b;                   // the sequence,
+  unsigned per_head;       // its units per kv head
+  DeviceSequence seq;
 };
 
 // Sum of v over the block (to every thread).
@@ -82,31 +84,41 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, Sc
 }
 
 // Units of all sequences.  `mine` keeps those of sequence threadIdx.x for find_unit.
+struct ThreadSequence {  // of sequence threadIdx.x (+ the block's size times the round)
+  DeviceSequence seq;
+  unsigned per_head;
+  template <int kRows>
+  __device__ __forceinline__ void load(const CacheAttention& a, unsigned b) {
+    per_head = 0;
+    if (b < a.c.batch) {
+      seq = load_sequence(a.c, b);
+      per_head = head_units<kRows>(a, seq);
+    }
+  }
+};
 template <int kRows, int kThreads>
 __device__ __forceinline__ unsigned long long all_units(const CacheAttention& a, ScheduleShared* sh,
-                                                        unsigned long long* mine) {
+                                                        ThreadSequence* mine) {
   unsigned long long n = 0;
-  *mine = 0;
-  for (unsigned b = threadIdx.x; b < a.c.batch; b += kThreads) {
-    const unsigned long long u =
-        static_cast<unsigned long long>(head_units<kRows>(a, load_sequence(a.c, b))) * a.c.kv_heads;
-    if (b < kThreads) *mine = u;
-    n += u;
+  mine->template load<kRows>(a, threadIdx.x);
+  n = mine->per_head;
+  for (unsigned b = threadIdx.x + kThreads; b < a.c.batch; b += kThreads) {
+    ThreadSequence t;
+    t.template load<kRows>(a, b);
+    n += t.per_head;
   }
-  return block_sum<kThreads>(n, sh);
+  return block_sum<kThreads>(n, sh) * a.c.kv_heads;
 }
 
-// The sequence that unit u (< all units) belongs to -> sh->seq, and u's place within it -> sh->rem.
+// The sequence that unit u (< all units) belongs to and u's place within it -> *sh.
 template <int kRows, int kThreads>
-__device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long long u, unsigned long long mine,
+__device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long long u, ThreadSequence mine,
                                           ScheduleShared* sh) {
   unsigned long long before = 0;  // units of the sequences of earlier rounds
   for (unsigned b0 = 0; b0 < a.c.batch; b0 += kThreads) {
-    const unsigned b = b0 + threadIdx.x;
-    if (b0) mine = b < a.c.batch
-                       ? static_cast<unsigned long long>(head_units<kRows>(a, load_sequence(a.c, b))) * a.c.kv_heads
-                       : 0ull;
-    unsigned long long v = mine;  // inclusive scan over the block
+    if (b0) mine.template load<kRows>(a, b0 + threadIdx.x);
+    const unsigned long long own = static_cast<unsigned long long>(mine.per_head) * a.c.kv_heads;
+    unsigned long long v = own;  // inclusive scan over the block
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long t = __shfl_up_sync(0xffffffffu, v, o);
@@ -122,9 +134,11 @@ __device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long
       if (w < static_cast<int>(threadIdx.x >> 5)) base += sh->sums[w];
       total += sh->sums[w];
     }
-    if (mine && base + v - mine <= u && u < base + v) {
-      sh->seq = static_cast<int>(b);
-      sh->rem = u - (base + v - mine);
+    if (own && base + v - own <= u && u < base + v) {
+      sh->b = static_cast<int>(b0 + threadIdx.x);
+      sh->rem = u - (base + v - own);
+      sh->per_head = mine.per_head;
+      sh->seq = mine.seq;
     }
     before += total;
     if (before > u) break;
@@ -155,10 +169,10 @@ struct ItemWalk {
   __device__ ItemWalk(const CacheAttention& a_, unsigned long long units, const ScheduleShared* sh)
       : a(a_), left(units), rem(0), b(0), per_head(0), head(0), tile(0), blocks(0), lo(0), hi(0), taken(0) {
     if (left == 0) return;
-    b = sh->seq;
+    b = sh->b;
     rem = sh->rem;
-    seq = load_sequence(a.c, b);
-    per_head = head_units<kRows>(a, seq);
+    seq = sh->seq;
+    per_head = sh->per_head;
     place();
     if (lo == hi) next();
   }
@@ -199,11 +213,43 @@ struct ItemWalk {
 
 // The pieces of cut items: a CTA has at most one that begins inside an item (slot 0) and one that
 // begins with it (slot 1).  A piece: kRows maxima (log2 units), kRows weight sums, kRows * DIM sums.
+// In front of the pieces lies a note per CTA that tells the merge kernel what it began, so that the
+// schedule is not worked out again.
+struct PieceNote {
+  unsigned ranges;  // CTAs whose ranges hold the rest of the item that this one began; 0: none
+  unsigned head, tile, rows;
+  int first;        // the sequence's first row
+  unsigned pad[3];
+};
+constexpr size_t kNotesBytes = 32768;  // for up to 1024 CTAs
+static_assert(sizeof(PieceNote) == 32, "notes");
 template <int kRows, int DIM>
 __host__ __device__ constexpr size_t piece_floats() { return static_cast<size_t>(kRows) * (DIM + 2); }
 template <int kRows, int DIM>
 __device__ __forceinline__ float* piece(const CacheAttention& a, unsigned cta, bool begins) {
-  return a.scratch + (2ull * cta + (begins ? 1u : 0u)) * piece_floats<kRows, DIM>();
+  return a.scratch + kNotesBytes / 4 + (2ull * cta + (begins ? 1u : 0u)) * piece_floats<kRows, DIM>();
+}
+__device__ __forceinline__ PieceNote* piece_note(const CacheAttention& a, unsigned cta) {
+  return reinterpret_cast<PieceNote*>(a.scratch) + cta;
+}
+// By one thread of every CTA of the grid: the note of a CTA whose range [u0, u1) ends inside an item that it
+// began (`item` the range's last; nullptr: there is none).
+template <int kRows>
+__device__ __forceinline__ void write_note(const CacheAttention& a, unsigned cta, unsigned busy,
+                                           unsigned long long units, unsigned long long u1, const ItemWalk<kRows>* item) {
+  PieceNote n = {};
+  if (item && item->lo == 0 && item->hi < item->blocks) {
+    const unsigned long long end = u1 + (item->blocks - item->hi);  // the item's last unit + 1
+    unsigned last = static_cast<unsigned>(min(static_cast<unsigned long long>(busy - 1), (end - 1) * busy / units));
+    while (range_begin(units, busy, last) > end - 1) --last;
+    while (last + 1 < busy && range_begin(units, busy, last + 1) <= end - 1) ++last;
+    n.ranges = last - cta;
+    n.head = item->head;
+    n.tile = item->tile;
+    n.rows = static_cast<unsigned>(item->seq.count) * a.group;
+    n.first = item->seq.first;
+  }
+  *piece_note(a, cta) = n;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
