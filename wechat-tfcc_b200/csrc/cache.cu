@@ -35,18 +35,10 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const CacheParam
   const unsigned lane = threadIdx.x & 31u, sub = lane / kLanes, l = lane % kLanes;
   const unsigned row = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (row >= p.rows) return;
-  const int b = sequence_of_row(p, row);
-  if (b < 0) return;
-  const DeviceSequence seq = load_sequence(p, b);
-  if (!seq.ok) return;
-  const int pos = seq.length - seq.count + (static_cast<int>(row) - seq.first);
-  if (pos < 0) return;
-  const int page = page_of(p, b, pos);
-  if (page < 0) return;
   const unsigned vectors = 2 * p.kv_heads;
   constexpr int kUnroll = 4;
-  for (unsigned v0 = blockIdx.y * kUnroll * kPer; v0 < vectors; v0 += gridDim.y * kUnroll * kPer) {
-    float4 f[kUnroll];
+  float4 f[kUnroll];
+  auto load = [&](unsigned v0) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const unsigned i = v0 + u * kPer + sub, head = i >> 1;
@@ -56,20 +48,43 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const CacheParam
         f[u] = __ldcs(reinterpret_cast<const float4*>(src + head * DIM) + l);
       }
     }
+  };
+  // the values do not depend on where they go: their loads run while the place is looked up
+  unsigned v0 = blockIdx.y * kUnroll * kPer;
+  load(v0);
+  const int b = sequence_of_row(p, row);
+  if (b < 0) return;
+  const DeviceSequence seq = load_sequence(p, b);
+  if (!seq.ok) return;
+  const int pos = seq.length - seq.count + (static_cast<int>(row) - seq.first);
+  if (pos < 0) return;
+  const int page = page_of(p, b, pos);
+  if (page < 0) return;
+  while (true) {
+    uint32_t c[kUnroll];
+    float scale[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const unsigned i = v0 + u * kPer + sub, head = i >> 1;
       uint32_t m = max_abs_bits(0u, f[u]);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const TokenQuant q(m);
+      c[u] = q.codes4(f[u]);
+      scale[u] = q.scale;
+    }
+    const unsigned at0 = v0;
+    v0 += gridDim.y * kUnroll * kPer;
+    if (v0 < vectors) load(v0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned i = at0 + u * kPer + sub, head = i >> 1;
       if (i < vectors) {
-        const TokenQuant q(m);
         const size_t at = cache_slot(p, page, head, pos);
-        int8_t* codes = ((i & 1u) ? p.values : p.keys) + at * DIM;
-        reinterpret_cast<uint32_t*>(codes)[l] = q.codes4(f[u]);
-        if (l == 0) ((i & 1u) ? p.value_scales : p.key_scales)[at] = q.scale;
+        reinterpret_cast<uint32_t*>(((i & 1u) ? p.values : p.keys) + at * DIM)[l] = c[u];
+        if (l == 0) ((i & 1u) ? p.value_scales : p.key_scales)[at] = scale[u];
       }
     }
+    if (v0 >= vectors) break;
   }
 }
 

@@ -600,7 +600,13 @@ int cache_attention(const CacheAttentionArgs& args) {
   a.scratch = args.max_length > kBlockKeys ? static_cast<float*>(args.workspace) : nullptr;
   const bool wide = args.cache.dim == 128;
   int st = TFCCB200_OK;
-  if (a.group <= kFewRows) {
+  // Whether a sequence has few rows or many is device data.  Where max_new says that there may be both
+  // kinds, both kernels are launched, unless all blocks together are so few that the second kernel
+  // and its merge cost more (about 10 us) than the many-rows kernel loses on the others (1.4 us
+  // per block and SM).
+  const bool only_few = static_cast<unsigned long long>(args.max_new) * a.group <= kFewRows;
+  const bool only_many = a.group > kFewRows || (!only_few && few_units_bound(args) * 14 <= 100ull * di->sm_count);
+  if (!only_many) {
     a.min_rows = 1;
     a.max_rows = kFewRows;
     if (few_rows_of(args) == 8)
@@ -609,8 +615,8 @@ int cache_attention(const CacheAttentionArgs& args) {
       st = wide ? launch_few<128, 16>(args, a, di->sm_count) : launch_few<64, 16>(args, a, di->sm_count);
     if (st != TFCCB200_OK) return st;
   }
-  if (static_cast<unsigned long long>(args.max_new) * a.group > kFewRows) {
-    a.min_rows = kFewRows + 1;
+  if (!only_few) {
+    a.min_rows = only_many ? 1 : kFewRows + 1;
     a.max_rows = 0xffffffffu;
     st = cache_attention_many(args, a, di->sm_count);
   }

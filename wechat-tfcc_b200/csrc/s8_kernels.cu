@@ -14,15 +14,15 @@ namespace tfccb200 {
 
 namespace {
 
-// One pass over x: THREADS threads share a row, each holding up to kHold 16-byte words of it in
-// registers between the maximum and the codes, so that the row is read from memory once; a row
-// longer than 4 * kHold * THREADS values is read a second time (from L2) for its tail.
-// The exact rounding costs about 15 instructions a value, which 5 bytes of traffic leave time for.
-template <int THREADS>
+// One pass over x: THREADS threads share a row, each holding up to kHold 16-byte words of it (or, rows
+// that do not start on 16 bytes, 4 * kHold single values) in registers between the maximum and the codes, so
+// that the row is read from memory once; what is left of a row longer than 4 * kHold * THREADS values
+// is read a second time, from L2.  Bound by memory for wide rows (8192 x 8192: XXX us, XXX TB/s of the
+// 5 bytes a value), by latency for few.
+template <int THREADS, bool kVec>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS)
 quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src, unsigned rows, unsigned cols,
-                       int8_t* __restrict__ codes, unsigned long long ld_codes, float* __restrict__ scales,
-                       bool vec) {
+                       int8_t* __restrict__ codes, unsigned long long ld_codes, float* __restrict__ scales) {
   constexpr int kHold = 4;
   constexpr int kBlock = THREADS < 128 ? 128 : THREADS;
   __shared__ uint32_t sh[kBlock / 32];
@@ -35,21 +35,27 @@ quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src,
   const bool live = row < rows;
   const float* p = src + (live ? row : 0) * ld_src;
   int8_t* out = codes + (live ? row : 0) * ld_codes;
+  // unit i of the row: 4 values (kVec) or 1
+  const unsigned units = !live ? 0 : (kVec ? cols / 4 : cols);
+  constexpr int kUnits = kVec ? kHold : 4 * kHold;
   float4 held[kHold];
   uint32_t m = 0;
-  const unsigned words = vec ? cols / 4 : 0;
-  if (live) {
+  if constexpr (kVec) {
 #pragma unroll
-    for (int u = 0; u < kHold; ++u) {
-      const unsigned i = t + u * THREADS;
-      held[u] = i < words ? __ldcs(reinterpret_cast<const float4*>(p) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    for (int u = 0; u < kHold; ++u)
+      held[u] = t + u * THREADS < units ? __ldcs(reinterpret_cast<const float4*>(p) + t + u * THREADS)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
 #pragma unroll
-    for (int u = 0; u < kHold; ++u) m = max_abs_bits(m, held[u]);
-    for (unsigned i = t + kHold * THREADS; i < words; i += THREADS)
-      m = max_abs_bits(m, reinterpret_cast<const float4*>(p)[i]);
-    for (unsigned i = words * 4 + t; i < cols; i += THREADS) m = max(m, abs_bits(p[i]));
+    for (int u = 0; u < kUnits; ++u) (&held[u / 4].x)[u % 4] = t + u * THREADS < units ? __ldcs(p + t + u * THREADS) : 0.f;
   }
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) m = max_abs_bits(m, held[u]);
+  for (unsigned i = t + kUnits * THREADS; i < units; i += THREADS) {
+    if constexpr (kVec) m = max_abs_bits(m, reinterpret_cast<const float4*>(p)[i]);
+    else m = max(m, abs_bits(p[i]));
+  }
+  if (kVec && live && cols / 4 * 4 + t < cols) m = max(m, abs_bits(p[cols / 4 * 4 + t]));
   if constexpr (THREADS >= 32) {
     m = __reduce_max_sync(0xffffffffu, m);
     if constexpr (THREADS > 32) {
@@ -64,14 +70,23 @@ quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src,
   if (!live) return;
   const TokenQuant q(m);
   if (t == 0) scales[row] = q.scale;
+  if constexpr (kVec) {
 #pragma unroll
-  for (int u = 0; u < kHold; ++u) {
-    const unsigned i = t + u * THREADS;
-    if (i < words) reinterpret_cast<uint32_t*>(out)[i] = q.codes4(held[u]);
+    for (int u = 0; u < kHold; ++u)
+      if (t + u * THREADS < units) reinterpret_cast<uint32_t*>(out)[t + u * THREADS] = q.codes4(held[u]);
+    for (unsigned i = t + kUnits * THREADS; i < units; i += THREADS)
+      reinterpret_cast<uint32_t*>(out)[i] = q.codes4(reinterpret_cast<const float4*>(p)[i]);
+    if (cols / 4 * 4 + t < cols) out[cols / 4 * 4 + t] = static_cast<int8_t>(q.code(p[cols / 4 * 4 + t]));
+  } else {
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+      const uint32_t c = q.codes4(held[u]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t + (4 * u + e) * THREADS < units) out[t + (4 * u + e) * THREADS] = static_cast<int8_t>(c >> (8 * e));
+    }
+    for (unsigned i = t + kUnits * THREADS; i < units; i += THREADS) out[i] = static_cast<int8_t>(q.code(p[i]));
   }
-  for (unsigned i = t + kHold * THREADS; i < words; i += THREADS)
-    reinterpret_cast<uint32_t*>(out)[i] = q.codes4(reinterpret_cast<const float4*>(p)[i]);
-  for (unsigned i = words * 4 + t; i < cols; i += THREADS) out[i] = static_cast<int8_t>(q.code(p[i]));
 }
 
 // ---- few tokens: memory-bound on the weights ------------------------------------------------------
@@ -294,16 +309,15 @@ int quantize_tokens(cudaStream_t stream, const float* src, unsigned long long ld
                     int8_t* codes, unsigned long long ld_codes, float* scales) {
   const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && ld_src % 4 == 0 &&
                    (reinterpret_cast<uintptr_t>(codes) & 3u) == 0 && ld_codes % 4 == 0;
+  auto run = [&](auto kernel, unsigned rows_per_block, unsigned threads) {
+    return launch_after_previous(kernel, dim3((rows + rows_per_block - 1) / rows_per_block), dim3(threads), 0, stream,
+                                 src, ld_src, rows, cols, codes, ld_codes, scales);
+  };
   cudaError_t e;
-  if (cols <= 512)
-    e = launch_after_previous(quantize_tokens_kernel<32>, dim3((rows + 3) / 4), dim3(128), 0, stream, src, ld_src,
-                              rows, cols, codes, ld_codes, scales, vec);
-  else if (cols <= 2048)
-    e = launch_after_previous(quantize_tokens_kernel<128>, dim3(rows), dim3(128), 0, stream, src, ld_src, rows, cols,
-                              codes, ld_codes, scales, vec);
-  else
-    e = launch_after_previous(quantize_tokens_kernel<512>, dim3(rows), dim3(512), 0, stream, src, ld_src, rows, cols,
-                              codes, ld_codes, scales, vec);
+  if (cols <= 512) e = vec ? run(quantize_tokens_kernel<32, true>, 4, 128) : run(quantize_tokens_kernel<32, false>, 4, 128);
+  else if (cols <= 2048) e = vec ? run(quantize_tokens_kernel<128, true>, 1, 128) : run(quantize_tokens_kernel<128, false>, 1, 128);
+  else if (cols <= 4096) e = vec ? run(quantize_tokens_kernel<256, true>, 1, 256) : run(quantize_tokens_kernel<256, false>, 1, 256);
+  else e = vec ? run(quantize_tokens_kernel<512, true>, 1, 512) : run(quantize_tokens_kernel<512, false>, 1, 512);
   if (e != cudaSuccess) return static_cast<int>(e);
   count_launch();
   return TFCCB200_OK;

@@ -7,8 +7,11 @@
 // the division is evaluated.  q = rint(x * fl(1/s)) is within one of the answer; the residual
 // r = x - q s is exact in fp32 (for |x| >= s it is a multiple of ulp(s) no larger than s, for
 // |x| < s either q = 0 or Sterbenz applies), so comparing |r| with s / 2 settles the rounding and
-// its ties.  A vector of zeros has s = 0 and codes 0; a vector that holds an infinity or a NaN
-// has s = NaN and codes 0, so whatever reads it back sees NaN instead of a plausible number.
+// its ties.  Almost every value takes four instructions: the product is rounded by adding
+// 1.5 * 2^23, whose low bits then are the code, and |r| < s / 2 confirms it; the others (within
+// rounding of a tie) go through code().  A vector of zeros has s = 0 and codes 0; a vector that holds an
+// infinity or a NaN has s = NaN and codes 0, so whatever reads it back sees NaN instead of a plausible
+// number.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -47,6 +50,21 @@ struct TokenQuant {
     return live ? __float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f)) : 0;
   }
   __device__ __forceinline__ uint32_t codes4(float4 v) const {
+    if (!live) return 0;
+    if (up == 1.0f) {
+      constexpr float kMagic = 12582912.f;
+      const float h = 0.5f * s;
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      uint32_t q[4];
+      bool sure = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float t = fmaf(x[i], inv, kMagic);
+        q[i] = __float_as_uint(t);
+        sure &= fabsf(fmaf(kMagic - t, s, x[i])) < h;
+      }
+      if (sure) return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    }
     const uint32_t a = code(v.x) & 0xff, b = code(v.y) & 0xff, c = code(v.z) & 0xff, d = code(v.w) & 0xff;
     return a | (b << 8) | (c << 16) | (d << 24);
   }

@@ -1016,6 +1016,9 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
             c_hi = c_lo + slice / 32;
           }
           if (row0 >= pM) c_hi = c_lo;  // no row of this warp exists
+          float* const c_first = reinterpret_cast<float*>(tgt.dst[0]);
+          const unsigned long long c_pitch = tgt.ldc;
+          const bool wide_rows = c_pitch % 2 == 0 && (reinterpret_cast<uintptr_t>(c_first) & 7u) == 0;
 #pragma unroll 1
           for (unsigned c = c_lo; c < c_hi; ++c) {
             const unsigned colb = col0 + c * 32;
@@ -1055,12 +1058,27 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
               epi_tma_store_block(out, lane, &tmapC, colb, row0, b);
             } else {
               __syncwarp();
-              const bool col_ok = colb + lane < pN;
-#pragma unroll 4
-              for (unsigned rr = 0; rr < 32; ++rr) {
-                const uint32_t v = out[rr * 32 + (((lane >> 2) ^ (rr & 7u)) << 2) + (lane & 3u)];
-                if (row0 + rr < pM && col_ok)
-                  tgt.dst[0][static_cast<unsigned long long>(row0 + rr) * tgt.ldc + colb + lane] = v;
+              const unsigned rows = min(32u, pM - row0);
+              if (wide_rows) {  // rows start on 8 bytes: half a warp per row
+                const unsigned l2 = 2 * (lane & 15u), r2 = lane >> 4;
+                const bool col_ok = colb + l2 < pN;
+                float2* dst = reinterpret_cast<float2*>(c_first + (row0 + r2) * c_pitch + colb + l2);
+#pragma unroll 8
+                for (unsigned rr = 0; rr < 32; rr += 2) {
+                  const unsigned r = rr + r2;
+                  const float2 v = *reinterpret_cast<const float2*>(out + r * 32 + (((l2 >> 2) ^ (r & 7u)) << 2) + (l2 & 3u));
+                  if (r < rows && col_ok) *dst = v;
+                  dst += c_pitch;
+                }
+              } else {
+                const bool col_ok = colb + lane < pN;
+                float* dst = c_first + row0 * c_pitch + colb + lane;
+#pragma unroll 8
+                for (unsigned r = 0; r < 32; ++r) {
+                  const uint32_t v = out[r * 32 + (((lane >> 2) ^ (r & 7u)) << 2) + (lane & 3u)];
+                  if (r < rows && col_ok) *dst = __uint_as_float(v);
+                  dst += c_pitch;
+                }
               }
               __syncwarp();
             }
