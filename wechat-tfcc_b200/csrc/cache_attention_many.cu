@@ -23,11 +23,15 @@
 //   warps 8-15  softmax, sums and output of 16 rows each.  Tensor memory is read and written in the
 //               layout of matrix fragments, two rows and every fourth pair of keys per thread: 64 scores
 //               and 64 sums fit the registers, a row's maximum and sum are two shuffles, and a
-//               thread reads the scales of 32 keys instead of 128.  (A thread per row with all of
-//               its 128 sums left no registers to overlap the exponentials with and read every scale:
-//               3.4 times slower.)
-// Bound by the tensor core (8 dim flops per row and key instead of the 4 counted) and, close behind,
-// by the issue slots of the softmax.
+//               thread reads the scales of 32 keys instead of 128
+// Bound by the tensor core: 8 dim flops per row and key instead of the 4 counted, at the rate the card
+// sustains on dense data.  4096 new tokens on 4096 cached ones, 32 / 8 heads of 128: 838 us, 492 TFLOP/s
+// counted, 984 executed (0.60 of the measured burst rate of bf16 products, 0.70 of the sustained one).  What was
+// measured on the way there (the same case): a thread per row with all of its 128 sums, two
+// tiles per CTA 1137; two threads per row 1193; this layout 955; products issued with precomputed
+// descriptors 932; items weighted in the schedule 870; scales in the order of their reading 838.
+// Slower: sixteen softmax warps 1088, products summed over four blocks in tensor memory 972, codes
+// through a ring of bulk copies 880, code loads two tiles ahead 930.
 //
 // Every wait is bounded: on expiry a status bit is raised and all roles run to their end.
 #include <cuda_runtime.h>
@@ -59,13 +63,21 @@ struct Item {  // what the roles need to know of an item; hi == 0 ends the walk
   unsigned pad[2];
 };
 
+// A block's 128 key (or value) scales in shared memory, in the order the softmax reads them: the 32 of the
+// keys 8 i + 2 t, + 1 of thread t of a quad together, and the quad's four groups on different banks.
+constexpr int kScalePitch = 36;
+__device__ __forceinline__ unsigned scale_place(unsigned key) {
+  return ((key >> 1) & 3u) * kScalePitch + (key >> 3) * 2 + (key & 1u);
+}
+
 template <int DIM>
 struct ManyLayout {
   static constexpr int kHalves = DIM / 64;               // 64-wide tiles of a row
   static constexpr int kOperand = kHalves * kTileBytes;  // 128 rows of K or V
   static constexpr int kRing = DIM == 128 ? 6 : 8;
   static constexpr int kScales = kRing * kOperand;       // 2 x {ks[128], vr[128]}
-  static constexpr int kItems = kScales + 2 * 1024;
+  static constexpr int kScaleBytes = 2 * 4 * kScalePitch * 4;
+  static constexpr int kItems = kScales + 2 * kScaleBytes;
   static constexpr int kBars = kItems + 2 * static_cast<int>(sizeof(Item));
   static constexpr int kNumBars = 30;
   static constexpr int kMisc = kBars + 8 * kNumBars;           // tensor memory address, abort flag, value factors
@@ -270,11 +282,12 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           top = min((top + 0x7fffffu) & 0x7f800000u, 0x7f000000u);  // up to a power of two
           const float up = kWeightTop / __uint_as_float(top);
           if (!wait(sc_empty + 8 * s, ((n >> 1) & 1u) ^ 1u, TFCCB200_DEV_TIMEOUT_CONVERT)) return false;
-          float* dst = reinterpret_cast<float*>(smem + L::kScales + s * 1024);
+          float* dst = reinterpret_cast<float*>(smem + L::kScales + s * L::kScaleBytes);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            dst[i * 32 + lane] = ks[i];
-            dst[128 + i * 32 + lane] = vs[i] * up;
+            const unsigned at = scale_place(i * 32 + lane);
+            dst[at] = ks[i];
+            dst[4 * kScalePitch + at] = vs[i] * up;
           }
           if (lane == 0) value_back[s] = __uint_as_float(top) * (1.f / kWeightTop);
           __syncwarp();
@@ -464,8 +477,9 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         constexpr bool kMask = decltype(mask)::value;
         const unsigned s = nb & 1u;
         const uint32_t t_s = rows_addr + L::kTmemS + s * 128;
-        // scales of this thread's keys 8 i + 2 t, + 1 in pairs, and (from 64 on) of their values
-        const uint64_t* scales = reinterpret_cast<const uint64_t*>(smem + L::kScales + s * 1024) + t;
+        // scales of this thread's keys 8 i + 2 t, + 1 for two i at a time, then of their values
+        const ulonglong2* ks_at = reinterpret_cast<const ulonglong2*>(smem + L::kScales + s * L::kScaleBytes) + t * (kScalePitch / 4);
+        const ulonglong2* vs_at = ks_at + kScalePitch;
         if (!wait(sc_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         if (!wait(s_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         ptx::tc_fence_after_sync();
@@ -478,7 +492,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint64_t ks = scales[4 * i];
+          const uint64_t ks = (i & 1) ? ks_at[i / 2].y : ks_at[i / 2].x;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float* e = &y[4 * i + 2 * k];
@@ -526,7 +540,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int c = 4 * ch + i;
-            const uint64_t vs = scales[64 + 4 * c];
+            const uint64_t vs = (c & 1) ? vs_at[c / 2].y : vs_at[c / 2].x;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const float2 e = unpair(fma2(pair(y[4 * c + 2 * k], y[4 * c + 2 * k + 1]), rs2[k], ref2[k]));
