@@ -409,6 +409,64 @@ def test_a_captured_step_follows_the_sequences(pkg, most):
     pkg.session.get_session(dev()).sync()
 
 
+def test_many_sequences(pkg):
+    """More sequences than a CTA has threads, most of them short, some empty, with and without new tokens."""
+    rng = np.random.default_rng(5)
+    news = [int(rng.integers(0, 3)) for _ in range(1100)]
+    lengths = [n + int(rng.integers(0, 40)) for n in news]
+    news[700], lengths[700] = 60, 700
+    lengths[1099] = 3000
+    s = Setup(pkg, news, lengths, 2, 64, 16, seed=13)
+    q = torch.randn(s.rows, 8 * 64, device=dev(), generator=s.g)
+    want, tol = expected(s, q, 8, 0.125, True)
+    compare(pkg.cache.attention(s.cache, q, s.starts, s.lens, s.table), want, tol, s.rows)
+    k, v = (torch.randn(s.rows, 128, device=dev(), generator=s.g) for _ in "kv")
+    pkg.cache.append(s.cache, k, v, s.starts, s.lens, s.table)
+    rk, rv = pkg.cache.read(s.cache, s.starts, s.lens, s.table, s.rows)
+    for x, r in ((k, rk), (v, rv)):
+        c, sc = reference_codes(x.view(-1, 64))
+        np.testing.assert_array_equal(r.view(-1, 64).cpu().numpy(), c.astype(np.float32) * sc[:, None])
+    pkg.session.get_session(dev()).sync()
+
+
+def test_a_call_without_new_tokens_leaves_everything(pkg):
+    s = Setup(pkg, [0, 0], [30, 500], 2, 64, 16, seed=14, pad_rows=5)
+    q = torch.randn(5, 4 * 64, device=dev())
+    for most in (1, 5):
+        out = torch.full((5, 256), 2.0, device=dev())
+        pkg.cache.attention(s.cache, q, s.starts, s.lens, s.table, max_new=most, out=out)
+        assert bool((out == 2.0).all())
+    before = s.cache.keys.clone()
+    kv = torch.randn(5, 128, device=dev())
+    pkg.cache.append(s.cache, kv, kv, s.starts, s.lens, s.table)
+    assert torch.equal(s.cache.keys, before)
+    pkg.session.get_session(dev()).sync()
+
+
+def test_graphs_replayed_side_by_side(pkg):
+    """Two captured calls with pieces in scratch, replayed on two streams at once."""
+    setups, graphs, outs, wants = [], [], [], []
+    for seed, news, lengths in ((20, [1, 1], [9000, 7000]), (21, [200], [6000]), (22, [1], [12000])):
+        s = Setup(pkg, news, lengths, 2, 128, 64, seed=seed)
+        q = torch.randn(s.rows, 8 * 128, device=dev(), generator=s.g)
+        wants.append(pkg.cache.attention(s.cache, q, s.starts, s.lens, s.table, max_new=max(news)))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pkg.cache.attention(s.cache, q, s.starts, s.lens, s.table, max_new=max(news)))
+        setups.append((s, q))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, want in zip(outs, wants):
+        assert torch.equal(out, want)
+    pkg.session.get_session(dev()).sync()
+
+
 def test_side_streams(pkg):
     s = Setup(pkg, [1, 90, 2], [500, 300, 7], 2, 128, 16, seed=12)
     q = torch.randn(s.rows, 6 * 128, device=dev(), generator=s.g)

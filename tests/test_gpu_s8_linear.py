@@ -212,6 +212,41 @@ def test_quantize_channels(pkg):
     assert codes.stride(0) % 16 == 0
 
 
+def test_linear_graphs_replayed_side_by_side(pkg):
+    """Each captured call keeps the codes of its own activations."""
+    _, _, b, sb, bias = operands(1, 2048, 512, 3)
+    graphs, outs, wants = [], [], []
+    for m in (3, 16, 300):
+        x = activations(m, 2048, m).to(dev())
+        wants.append(pkg.quantization.linear(x, b, sb, bias))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pkg.quantization.linear(x, b, sb, bias))
+        graphs.append((g, x))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(50):
+        for st, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, want in zip(outs, wants):
+        assert torch.equal(out, want)
+
+
+def test_weights_written_just_before_are_seen(pkg):
+    """The few-token product asks for its weights before it waits for the kernel ahead: what an earlier kernel of
+    the stream wrote into them has to be there."""
+    _, _, b, sb, _ = operands(1, 4096, 2048, 5)
+    new = torch.randint(-127, 128, tuple(b.shape), dtype=torch.int8, device=dev())
+    x = activations(7, 4096, 6).to(dev())
+    codes, scales = pkg.quantization.quantize_tokens(x)
+    for w in (new, -new, new // 2) * 4:
+        b.copy_(w)
+        got = pkg.quantization.linear(x, b, sb)
+        check(got, codes, scales, w, sb, None)
+
+
 def test_linear_in_a_graph_and_on_a_side_stream(pkg):
     _, _, b, sb, bias = operands(1, 512, 640, 3)
     x = activations(20, 512, 4).to(dev())

@@ -171,7 +171,7 @@ def attention(cache: PagedCache, q: torch.Tensor, starts: torch.Tensor, lengths:
         scale = 1.0 / float(cache.dim) ** 0.5
     sess, stream, guard = launch_context(cache.device)
     with guard:
-        ws_ptr, ws_len = sess.workspace_on(
+        ws_ptr, ws_len, _owner = sess.workspace_on(
             lib.tfccb200_cache_attention_workspace(cache._ref, batch, rows, heads, max_new, max_length), stream)
         check(lib.tfccb200_cache_attention_f32(stream, cache._ref, q.data_ptr(), ldq, out.data_ptr(),
                                                ldo, ps, pl, pt, batch, width, rows, heads, max_new, max_length,

@@ -1,8 +1,9 @@
 // Attention over the paged 8-bit cache for many rows per kv head: chunks of prompts, tcgen05.
 //
 // An item is 128 query rows of one kv head (the rows of one MMA) against a run of 128-key blocks.
-// Arithmetic as in cache_attention.cu: K, V exact in fp16, Q and the weights as two fp16 terms each, so
-// per block
+// K and V are exact in fp16, and the fp32 operands are split into two fp16 terms each, x = hi + lo with 11 bits:
+// q per row after scaling by a power of two, and the weights w_j = p_j vs_j as in
+// cache_attention.cu.  Per block
 //   S = Q_hi K^T + Q_lo K^T          A from tensor memory, K from shared memory, fp32 sums
 //   P = exp2(S ks - m) vs            hi and lo terms go back over S
 //   O_block = P_hi V + P_lo V        A from tensor memory, V as it lies (MN-major)

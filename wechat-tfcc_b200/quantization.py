@@ -376,7 +376,7 @@ def linear(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch
     out = torch.empty(x.shape[:-1] + (n,), dtype=torch.float32, device=x.device)
     sess, stream, guard = launch_context(x.device)
     with guard:
-        ws_ptr, ws_len = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k), stream)
+        ws_ptr, ws_len, _owner = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k), stream)
         check(lib.tfccb200_qlinear_f32(stream, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias,
                                        out.data_ptr(), m, n, k, ACTIVATIONS[activation], ws_ptr, ws_len,
                                        sess.status_ptr))

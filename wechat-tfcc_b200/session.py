@@ -34,11 +34,19 @@ class Session:
         return self._status.data_ptr()
 
     def workspace_on(self, nbytes: int, stream_ptr: int):
-        """:meth:`workspace` for a caller that already has the current stream's handle."""
+        """``(pointer, bytes, owner)`` of scratch for one call on the current stream, whose handle the
+        caller already has: the stream's buffer (:meth:`workspace`), or under capture one of the call's own, so
+        that captured graphs, which may be replayed side by side, share none.  ``owner`` has to live
+        until the call is launched."""
+        if nbytes == 0:
+            return None, 0, None
+        if _capturing():
+            own = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            return own.data_ptr(), nbytes, own
         ws = self._workspaces.get(stream_ptr)
-        if nbytes and ws is not None and ws.numel() >= nbytes:
-            return ws.data_ptr(), ws.numel()
-        return self.workspace(nbytes)
+        if ws is not None and ws.numel() >= nbytes:
+            return ws.data_ptr(), ws.numel(), ws
+        return *self.workspace(nbytes), None
 
     def workspace(self, nbytes: int):
         """Scratch of at least ``nbytes`` for calls on the current stream (grown
@@ -90,6 +98,7 @@ class _NoGuard:
 
 
 _NO_GUARD = _NoGuard()
+_capturing = torch.cuda.is_current_stream_capturing
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
