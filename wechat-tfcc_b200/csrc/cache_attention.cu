@@ -94,6 +94,15 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint4 a, uint32_t b0, uin
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint4 a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Where 16-byte chunk `c` of code row `r` of a stage lies.  K rows are read by four lanes per row,
 // V rows by lanes that share a chunk over four rows of one parity; both orders then touch eight different
 // chunks of a 128-byte line in every quarter of a warp's access.
@@ -272,11 +281,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
     }
     __syncthreads();
 
-    float o[kTiles][4];
+    float o[kTiles][ROWS / 4];  // [tile i][2 h + c]: column kTiles (2 t + c) + i of row g + 8 h
 #pragma unroll
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+      for (int j = 0; j < ROWS / 4; ++j) o[i][j] = 0.f;
     float top[ROWS / 8], sum[ROWS / 8], vref = kValueFloor, vup = kWeightTop / kValueFloor;
 #pragma unroll
     for (int h = 0; h < ROWS / 8; ++h) top[h] = -INFINITY, sum[h] = 0.f;
@@ -392,10 +401,6 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
           for (int i = 0; i < kTiles; ++i) {
             o[i][2 * h] *= f * vf;
             o[i][2 * h + 1] *= f * vf;
-            if constexpr (ROWS == 8) {
-              o[i][2] *= f * vf;
-              o[i][3] *= f * vf;
-            }
           }
         }
       }
@@ -452,8 +457,18 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
         const uint32_t x1[4] = {codes_low(b01), codes_high(b01), codes_low(b23), codes_high(b23)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          mma_f16(o[w * 4 + i], pa, x0[i], x1[i]);
-          if constexpr (ROWS == 16) mma_f16(o[w * 4 + i], pb, x0[i], x1[i]);
+          // from zero, and added in fp32: the instruction's own accumulation narrows without rounding
+          // to nearest, which over thousands of keys doubled the error (6e-7 to 1.2e-6 at 65536)
+          float d[4];
+          mma_f16_zero(d, pa, x0[i], x1[i]);
+          if constexpr (ROWS == 8) {
+            o[w * 4 + i][0] += d[0] + d[2];
+            o[w * 4 + i][1] += d[1] + d[3];
+          } else {
+            mma_f16(d, pb, x0[i], x1[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[w * 4 + i][j] += d[j];
+          }
         }
       }
       __syncwarp();  // the stage may be overwritten
@@ -489,7 +504,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
             float4 y;
             float* yy = &y.x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) yy[k] = ROWS == 8 ? o[i + k][c] + o[i + k][2 + c] : o[i + k][2 * h + c];
+            for (int k = 0; k < 4; ++k) yy[k] = o[i + k][2 * h + c];
             *reinterpret_cast<float4*>(dst + (g + 8 * h) * DIM + kTiles * (2 * t + c) + i) = y;
           }
     }
