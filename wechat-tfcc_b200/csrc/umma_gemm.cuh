@@ -980,7 +980,9 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
           // fp32 results from the exact int32 sums: one column block of 32 after the other goes
           // through a staging block of the warp and leaves by TMA store (or, for rows that are no
           // multiple of 16 bytes, by 128-byte row segments).  The CTA's last tile stages in the
-          // dead ring, all blocks side by side, so that no store waits for another.
+          // dead ring, all blocks side by side, so that no store waits for another.  Column factors are
+          // read four at a time from the warp's copy in shared memory: passing them between lanes
+          // took two shuffles per value and, with erff, made 4096x4096x16384 440 us instead of 207.
           const int act = tgt.activation;
           const bool last_tile = si + 1 == num_segments;
           unsigned c_lo = 0, c_hi = BN / 32;
