@@ -50,10 +50,10 @@ class PagedCache:
                                      (value_scales, "value_scales", torch.float32, shape[:3])):
             if not isinstance(t, torch.Tensor) or t.shape != want:
                 raise exceptions.InvalidArgumentError(f"{name}: expected shape {tuple(want)}")
-            if t.dtype != dtype:
+            if t.dtype is not dtype:
                 raise exceptions.NotImplementedError(f"{name}: implemented for {dtype}, got {t.dtype}")
         for t in (keys, key_scales, values, value_scales):
-            if not t.is_cuda or t.device != device or not t.is_contiguous():
+            if not t.is_cuda or t.get_device() != device.index or not t.is_contiguous():
                 raise exceptions.InvalidArgumentError("the cache's tensors must be contiguous CUDA tensors on one device")
         self.pages, self.kv_heads, self.page_size, self.dim = shape
         if self.dim not in (64, 128):
@@ -81,8 +81,8 @@ def _sequences(cache, starts, lengths, table):
         raise exceptions.InvalidArgumentError("cache must be a PagedCache")
     device = cache.device
     for t, name, rank in ((starts, "starts", 1), (lengths, "lengths", 1), (table, "table", 2)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != rank or t.numel() == 0 or \
-                t.device != device or not t.is_contiguous():
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != rank or t.numel() == 0 or \
+                not t.is_cuda or t.get_device() != device.index or not t.is_contiguous():
             raise exceptions.InvalidArgumentError(f"{name}: expected a contiguous int32 tensor of rank {rank} on {cache.device}")
     batch = lengths.shape[0]
     if starts.shape[0] != batch + 1 or table.shape[0] != batch:
@@ -92,14 +92,15 @@ def _sequences(cache, starts, lengths, table):
 
 def _packed(t, name, rows, width, device):
     """Row pitch of a [rows, width] float32 tensor with contiguous rows (a column slice will do)."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[1] != width or (rows is not None and t.shape[0] != rows) \
-            or t.shape[0] == 0:
+    shape = t.shape if isinstance(t, torch.Tensor) else ()
+    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows) or shape[0] == 0:
         raise exceptions.InvalidArgumentError(f"{name}: expected a [{'rows' if rows is None else rows}, {width}] tensor")
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         raise exceptions.NotImplementedError(f"{name}: implemented for float32, got {t.dtype}")
-    if t.device != device or t.stride(1) != 1:
+    pitch, step = t.stride()
+    if not t.is_cuda or t.get_device() != device.index or step != 1:
         raise exceptions.InvalidArgumentError(f"{name}: rows must be contiguous, on {device}")
-    return width if t.shape[0] == 1 else t.stride(0)
+    return width if shape[0] == 1 else pitch
 
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor,
@@ -128,11 +129,12 @@ def read(cache: PagedCache, starts: torch.Tensor, lengths: torch.Tensor, table: 
     if out is None:
         if rows <= 0:
             raise exceptions.InvalidArgumentError("rows must be positive")
-        out = (torch.empty(rows, cols, dtype=torch.float32, device=cache.device),
-               torch.empty(rows, cols, dtype=torch.float32, device=cache.device))
-    k, v = out
-    ldk = _packed(k, "out[0]", rows, cols, cache.device)
-    ldv = _packed(v, "out[1]", rows, cols, cache.device)
+        k, v = cache.key_scales.new_empty((rows, cols)), cache.key_scales.new_empty((rows, cols))
+        ldk = ldv = cols
+    else:
+        k, v = out
+        ldk = _packed(k, "out[0]", rows, cols, cache.device)
+        ldv = _packed(v, "out[1]", rows, cols, cache.device)
     sess, stream, guard = launch_context(cache.device)
     with guard:
         check(lib.tfccb200_cache_read_f32(stream, cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv,
@@ -159,8 +161,9 @@ def attention(cache: PagedCache, q: torch.Tensor, starts: torch.Tensor, lengths:
     rows, cols = q.shape
     ldq = _packed(q, "q", None, cols, cache.device)
     if out is None:
-        out = torch.empty(rows, cols, dtype=torch.float32, device=cache.device)
-    ldo = _packed(out, "out", rows, cols, cache.device)
+        out, ldo = q.new_empty((rows, cols)), cols
+    else:
+        ldo = _packed(out, "out", rows, cols, cache.device)
     max_new = rows if max_new is None else max_new
     max_length = width * cache.page_size if max_length is None else max_length
     if max_new <= 0 or max_length <= 0:

@@ -265,19 +265,20 @@ def _rows(t, name, dtype):
     contiguous and whose rows are evenly spaced."""
     if not isinstance(t, torch.Tensor) or t.dim() < 2 or t.numel() == 0:
         raise exceptions.InvalidArgumentError(f"invalid tensor {name}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise exceptions.NotImplementedError(f"{name}: implemented for {dtype}, got {t.dtype}")
     if not t.is_cuda:
         raise exceptions.InvalidArgumentError(f"{name} must be a CUDA tensor")
-    if t.dim() == 2:
-        rows, cols = t.shape
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
         pitch, step = t.stride()
         if rows == 1:
             pitch = max(pitch, cols)  # the stride of a single row says nothing
         if (cols != 1 and step != 1) or pitch < cols:
             raise exceptions.InvalidArgumentError(f"{name}: rows must be contiguous and must not overlap")
         return pitch, rows, cols
-    shape, stride = t.shape, t.stride()
+    stride = t.stride()
     cols = shape[-1]
     rows, pitch = shape[-2], stride[-2]
     for d in range(t.dim() - 3, -1, -1):
@@ -294,10 +295,10 @@ def _rows(t, name, dtype):
     return pitch, rows, cols
 
 
-def _vector(t, name, size, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or \
-            t.numel() != size or not t.is_contiguous():
-        raise exceptions.InvalidArgumentError(f"invalid tensor {name}: expected {size} contiguous float32 on {device}")
+def _vector(t, name, size, like):
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.numel() != size or \
+            not t.is_contiguous() or not t.is_cuda or t.get_device() != like.get_device():
+        raise exceptions.InvalidArgumentError(f"invalid tensor {name}: expected {size} contiguous float32 on {like.device}")
     return t.data_ptr()
 
 
@@ -343,14 +344,14 @@ def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     ldb, kb, n = _rows(b, "b", torch.int8)
     if b.dim() != 2 or kb != k:
         raise exceptions.InvalidArgumentError("tensor a and b don't match")
-    if b.device != a.device:
+    if b.get_device() != a.get_device():
         raise exceptions.InvalidArgumentError("operands live on different devices")
     if activation not in ACTIVATIONS or path not in PATHS:
         raise exceptions.InvalidArgumentError("unknown activation or path")
-    sa = _vector(a_scales, "a_scales", m, a.device)
-    sb = _vector(b_scales, "b_scales", n, a.device)
-    sbias = None if bias is None else _vector(bias, "bias", n, a.device)
-    out = torch.empty(list(a.shape[:-1]) + [n], dtype=torch.float32, device=a.device)
+    sa = _vector(a_scales, "a_scales", m, a)
+    sb = _vector(b_scales, "b_scales", n, a)
+    sbias = None if bias is None else _vector(bias, "bias", n, a)
+    out = a.new_empty(a.shape[:-1] + (n,), dtype=torch.float32)
     sess, stream, guard = launch_context(a.device)
     with guard:
         check(lib.tfccb200_qgemm_scaled_s8(stream, a.data_ptr(), lda, sa, b.data_ptr(), ldb,
@@ -367,13 +368,13 @@ def linear(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch
     ldb, kb, n = _rows(b, "b", torch.int8)
     if b.dim() != 2 or kb != k:
         raise exceptions.InvalidArgumentError("tensor x and b don't match")
-    if b.device != x.device:
+    if b.get_device() != x.get_device():
         raise exceptions.InvalidArgumentError("operands live on different devices")
     if activation not in ACTIVATIONS:
         raise exceptions.InvalidArgumentError("unknown activation")
-    sb = _vector(b_scales, "b_scales", n, x.device)
-    sbias = None if bias is None else _vector(bias, "bias", n, x.device)
-    out = torch.empty(x.shape[:-1] + (n,), dtype=torch.float32, device=x.device)
+    sb = _vector(b_scales, "b_scales", n, x)
+    sbias = None if bias is None else _vector(bias, "bias", n, x)
+    out = x.new_empty(x.shape[:-1] + (n,))
     sess, stream, guard = launch_context(x.device)
     with guard:
         ws_ptr, ws_len, _owner = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k), stream)
