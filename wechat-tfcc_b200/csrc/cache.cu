@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const CacheParams 
       if (i < vectors && page >= 0) {
         const size_t at = cache_slot(p, page, head, pos);
         c[u] = __ldcs(reinterpret_cast<const uint32_t*>(((i & 1u) ? p.values : p.keys) + at * DIM) + l);
-        s[u] = __ldg(((i & 1u) ? p.value_scales : p.key_scales) + at);
+        s[u] = ((i & 1u) ? p.value_scales : p.key_scales)[at];
       }
     }
 #pragma unroll

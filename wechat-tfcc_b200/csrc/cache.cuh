@@ -6,7 +6,9 @@
 //            sequence b, lengths[b] the tokens it has in the cache with the new ones, and
 //            position p of it lies in page table[b][p / page_size], slot p % page_size.
 // All three arrays are device data that the host never sees, so every kernel checks what it reads
-// before it uses it as an index: see DeviceSequence and page_of.
+// before it uses it as an index: see DeviceSequence and page_of.  All of it, and what the kernels read of
+// the cache, is read with ordinary loads: a kernel may be resident before the one that writes them is done,
+// and loads through the read-only path are only defined for data constant over a kernel's life.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -43,9 +45,9 @@ struct DeviceSequence {
 };
 __device__ __forceinline__ DeviceSequence load_sequence(const CacheParams& p, unsigned b) {
   DeviceSequence s;
-  s.first = __ldg(p.starts + b);
-  const int end = __ldg(p.starts + b + 1);
-  s.length = __ldg(p.lengths + b);
+  s.first = p.starts[b];
+  const int end = p.starts[b + 1];
+  s.length = p.lengths[b];
   s.ok = s.first >= 0 && end >= s.first && static_cast<unsigned>(end) <= p.rows &&
          static_cast<unsigned>(end - s.first) <= p.max_new && s.length >= 0 &&
          static_cast<unsigned>(s.length) <= p.max_length;
@@ -63,7 +65,7 @@ __device__ __forceinline__ void check_all_sequences(const CacheParams& p) {
 
 // Page of position `pos` (< length <= table_width * page_size) of sequence b, or -1.
 __device__ __forceinline__ int page_of(const CacheParams& p, unsigned b, unsigned pos) {
-  const int page = __ldg(p.table + static_cast<size_t>(b) * p.table_width + (pos >> p.page_shift));
+  const int page = p.table[static_cast<size_t>(b) * p.table_width + (pos >> p.page_shift)];
   if (page < 0 || static_cast<unsigned>(page) >= p.pages) {
     raise_status(p.status, TFCCB200_DEV_BAD_PAGE);
     return -1;
@@ -84,10 +86,10 @@ __device__ __forceinline__ size_t cache_slot(const CacheParams& p, int page, uns
 __device__ __forceinline__ int sequence_of_row(const CacheParams& p, unsigned row) {
   unsigned n = 0;
   for (unsigned i = threadIdx.x & 31u; i < p.batch; i += 32)
-    n += static_cast<long long>(__ldg(p.starts + i + 1)) <= static_cast<long long>(row) ? 1u : 0u;
+    n += static_cast<long long>(p.starts[i + 1]) <= static_cast<long long>(row) ? 1u : 0u;
   n = __reduce_add_sync(0xffffffffu, n);
   if (n >= p.batch) return -1;
-  const int first = __ldg(p.starts + n), end = __ldg(p.starts + n + 1);
+  const int first = p.starts[n], end = p.starts[n + 1];
   return static_cast<long long>(first) <= static_cast<long long>(row) &&
                  static_cast<long long>(row) < static_cast<long long>(end)
              ? static_cast<int>(n)

@@ -87,21 +87,21 @@ static __global__ void __launch_bounds__(256) cache_attention_merge_kernel(const
   for (unsigned e = (blockIdx.y * 256 + threadIdx.x) * 4; e < ROWS * DIM; e += gridDim.y * 1024) {
     const unsigned r = e / DIM, d = e % DIM, row = note.tile * ROWS + r;
     if (row >= note.rows) continue;
-    const float m1 = __ldg(p1 + r);
+    const float m1 = p1[r];
     float m = m1;
 #pragma unroll 8
-    for (unsigned k = 0; k < more; ++k) m = fmaxf(m, __ldg(p0 + k * kPitch + r));
+    for (unsigned k = 0; k < more; ++k) m = fmaxf(m, p0[k * kPitch + r]);
     const float base = m == -INFINITY ? 0.f : m;
     float f = exp2_fast(m1 - base);
-    float l = f * __ldg(p1 + ROWS + r);
-    const float4 y1 = __ldg(reinterpret_cast<const float4*>(p1 + 2 * ROWS + e));
+    float l = f * p1[ROWS + r];
+    const float4 y1 = *reinterpret_cast<const float4*>(p1 + 2 * ROWS + e);
     float4 acc = make_float4(f * y1.x, f * y1.y, f * y1.z, f * y1.w);
 #pragma unroll 8
     for (unsigned k = 0; k < more; ++k) {
       const float* p = p0 + k * kPitch;
-      const float4 y = __ldg(reinterpret_cast<const float4*>(p + 2 * ROWS + e));
-      f = exp2_fast(__ldg(p + r) - base);
-      l = fmaf(f, __ldg(p + ROWS + r), l);
+      const float4 y = *reinterpret_cast<const float4*>(p + 2 * ROWS + e);
+      f = exp2_fast(p[r] - base);
+      l = fmaf(f, p[ROWS + r], l);
       acc.x = fmaf(f, y.x, acc.x); acc.y = fmaf(f, y.y, acc.y);
       acc.z = fmaf(f, y.z, acc.z); acc.w = fmaf(f, y.w, acc.w);
     }

@@ -270,8 +270,8 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
               const int page = page_of(a.c, it.b, pos);
               if (page >= 0) {
                 const size_t at = cache_slot(a.c, page, it.head, pos);
-                ks[i] = __ldg(a.c.key_scales + at);
-                vs[i] = __ldg(a.c.value_scales + at);
+                ks[i] = a.c.key_scales[at];
+                vs[i] = a.c.value_scales[at];
               } else {  // a page that does not exist shows as NaN
                 ks[i] = vs[i] = __uint_as_float(0x7fffffffu);
               }
@@ -352,7 +352,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           const uint4* p = reinterpret_cast<const uint4*>(src + (pg >= 0 ? cache_slot(a.c, pg, it.head, key0 + r) : 0) * DIM);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
-            ahead[g * L::kHalves + h] = pg >= 0 ? __ldg(p + h * 4 + c4) : make_uint4(0u, 0u, 0u, 0u);
+            ahead[g * L::kHalves + h] = pg >= 0 ? p[h * 4 + c4] : make_uint4(0u, 0u, 0u, 0u);
         }
       };
       load(0);
@@ -409,7 +409,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
               a.q + a.ldq * (static_cast<size_t>(it.first) + tok) + static_cast<size_t>(hd) * DIM) + t;
 #pragma unroll
           for (int i = 0; i < DIM / 8; ++i) {
-            const float2 x = live ? __ldg(q + 4 * i) : make_float2(0.f, 0.f);
+            const float2 x = live ? q[4 * i] : make_float2(0.f, 0.f);
             f[k][2 * i] = x.x * a.scale;
             f[k][2 * i + 1] = x.y * a.scale;
           }

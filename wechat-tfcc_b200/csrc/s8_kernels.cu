@@ -22,8 +22,8 @@ namespace {
 // 256 threads a row and 27 with 512; 8192 x 8192 64 us (5.2 TB/s).  Few rows are bound by latency (1.5 us).
 template <int THREADS, bool kVec>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS)
-quantize_tokens_kernel(const float* __restrict__ src, unsigned long long ld_src, unsigned rows, unsigned cols,
-                       int8_t* __restrict__ codes, unsigned long long ld_codes, float* __restrict__ scales) {
+quantize_tokens_kernel(const float* src, unsigned long long ld_src, unsigned rows, unsigned cols,
+                       int8_t* codes, unsigned long long ld_codes, float* scales) {
   constexpr int kHold = 4;
   constexpr int kBlock = THREADS < 128 ? 128 : THREADS;
   __shared__ uint32_t sh[kBlock / 32];
@@ -249,8 +249,8 @@ s8_few_kernel(const __grid_constant__ S8GemmArgs a, unsigned splits) {
       v += o;
     }
     if (n < a.N) {
-      float y = static_cast<float>(v) * __ldg(a.a_scales + m);
-      y = fmaf(y, __ldg(a.b_scales + n), a.bias ? __ldg(a.bias + n) : 0.f);
+      float y = static_cast<float>(v) * a.a_scales[m];
+      y = fmaf(y, a.b_scales[n], a.bias ? a.bias[n] : 0.f);
       a.C[static_cast<size_t>(m) * a.N + n] = apply_activation(y, a.activation);
     }
   }

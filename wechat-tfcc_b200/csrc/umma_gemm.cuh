@@ -962,12 +962,12 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constan
         float* const terms = reinterpret_cast<float*>(bar_gen + Cfg::kBarrierBytes) + (warp - Cfg::kFirstEpilogueWarp) * 2 * BN;
         if constexpr (kKind == ptx::MmaKind::S8) {
           // the tile's row and column factors, fetched while the mainloop runs
-          row_scale = row_ok ? __ldg(p.a_scales + row) : 0.f;
+          row_scale = row_ok ? p.a_scales[row] : 0.f;
           if (row0 < pM) {
             for (unsigned i = lane; i < BN; i += 32) {
               const unsigned col = col0 + i;
-              terms[i] = col < pN ? __ldg(p.b_scales + col) : 0.f;
-              terms[BN + i] = (pbias && col < pN) ? __ldg(pbias + col) : 0.f;
+              terms[i] = col < pN ? p.b_scales[col] : 0.f;
+              terms[BN + i] = (pbias && col < pN) ? pbias[col] : 0.f;
             }
           }
           __syncwarp();
