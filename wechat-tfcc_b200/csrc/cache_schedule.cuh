@@ -115,6 +115,9 @@ template <int kRows, int kThreads>
 __device__ __forceinline__ void find_unit(const CacheAttention& a, unsigned long long u, ThreadSequence mine,
                                           ScheduleShared* sh) {
   unsigned long long before = 0;  // units of the sequences of earlier rounds
+  // (stays so only if the lengths change while the kernel reads them, which the caller must not let happen
+  // and which must not send a walk beyond the arrays)
+  if (threadIdx.x == 0) sh->b = -1;
   for (unsigned b0 = 0; b0 < a.c.batch; b0 += kThreads) {
     if (b0) mine.template load<kRows>(a, b0 + threadIdx.x);
     const unsigned long long own = static_cast<unsigned long long>(mine.per_head) * a.c.kv_heads;
@@ -170,6 +173,10 @@ struct ItemWalk {
       : a(a_), left(units), rem(0), b(0), per_head(0), head(0), tile(0), blocks(0), lo(0), hi(0), taken(0) {
     if (left == 0) return;
     b = sh->b;
+    if (b < 0) {
+      left = 0;
+      return;
+    }
     rem = sh->rem;
     seq = sh->seq;
     per_head = sh->per_head;
@@ -201,10 +208,14 @@ struct ItemWalk {
       while (rem >= static_cast<unsigned long long>(per_head) * a.c.kv_heads) {
         rem = 0;
         do {
-          ++b;
+          // units are left, so a sequence that has some follows (unless lengths change under the kernel)
+          if (static_cast<unsigned>(++b) >= a.c.batch) {
+            left = 0;
+            return;
+          }
           seq = load_sequence(a.c, b);
           per_head = head_units<kRows>(a, seq);
-        } while (per_head == 0);  // units are left, so a sequence that has some follows
+        } while (per_head == 0);
       }
       place();
     } while (lo == hi);
