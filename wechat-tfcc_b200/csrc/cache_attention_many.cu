@@ -299,9 +299,12 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
     } else if (warp == 2) {
       // ======================= walker =======================
       unsigned n = 0;
+      // An item's place is free when the softmax takes it up, which may be a whole item later: the limit
+      // grows with the range (20 us a block, several times what one takes).
+      const Waiter wait_item{abort_flag, a.c.status, timeout_ns + 20000ull * (u1 - u0)};
       auto put = [&](const Item& it) {
         const unsigned s = n & 1u;
-        if (!wait(it_empty + 8 * s, ((n >> 1) & 1u) ^ 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
+        if (!wait_item(it_empty + 8 * s, ((n >> 1) & 1u) ^ 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         if (lane == 0) {
           *reinterpret_cast<Item*>(smem + L::kItems + s * sizeof(Item)) = it;
           ptx::mbar_arrive(it_full + 8 * s);
