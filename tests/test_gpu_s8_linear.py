@@ -266,3 +266,15 @@ def test_linear_in_a_graph_and_on_a_side_stream(pkg):
         static.copy_(fresh)
         graph.replay()
         assert torch.equal(out, pkg.quantization.linear(fresh, b, sb, bias))
+
+
+@pytest.mark.parametrize("m,path", [(4, "auto"), (200, "umma"), (200, "umma2"), (200, "simt")])
+@pytest.mark.parametrize("activation", [None, "gelu"])
+def test_results_beyond_the_range_are_infinite(pkg, m, path, activation):
+    # 64 * 127 * 127 * 1e20 * 1e20 passes the largest float; gelu(+inf) = inf.  Column 1 is an exact zero.
+    a = torch.full((m, 64), 127, dtype=torch.int8, device="cuda")
+    b = torch.zeros(64, 16, dtype=torch.int8, device="cuda")
+    b[:, 0] = 127
+    s = torch.full((m,), 1e20, device="cuda")
+    out = pkg.quantization.matmul_scaled(a, s, b, torch.full((16,), 1e20, device="cuda"), activation=activation, path=path)
+    assert bool((out[:, 0] == math.inf).all()) and bool((out[:, 1:] == 0).all())

@@ -31,8 +31,8 @@ __device__ __forceinline__ float gelu_erfc(float v) {
   q = fmaf(q, t, 1.421413741f);
   q = fmaf(q, t, -0.284496736f);
   q = fmaf(q, t, 0.254829592f);
-  const float w = v * (0.5f * q * t * e);  // v erfc(z) / 2
-  return v >= 0.f ? v - w : w;  // (NaN takes the second branch and stays NaN)
+  const float h = 0.5f * q * t * e;  // erfc(z) / 2
+  return v * (v >= 0.f ? 1.f - h : h);  // (a factor, not a difference: infinity stays infinity)
 }
 
 __device__ __forceinline__ float apply_activation(float v, int activation) {
