@@ -603,6 +603,8 @@ TFCCB200_API size_t tfccb200_qlinear_workspace(unsigned M, unsigned K);
  * of the row's sequence up to its own position (causal) or all of them; a row that sees none is
  * 0.  max_new and max_length bound the new and cached tokens of one sequence; the launch is shaped
  * by them, and a sequence that exceeds them is passed over with TFCCB200_DEV_BAD_SEQUENCE.
+ * (max_new * heads / kv_heads / 128 + 1) * (max_length / 128 + 4) has to fit 32 bits.  starts, lengths
+ * and table must not change while a call runs.
  * workspace: tfccb200_cache_attention_workspace bytes, 256-byte aligned.
  */
 typedef struct tfccb200_cache {

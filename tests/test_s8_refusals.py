@@ -111,3 +111,17 @@ def test_python_checks_refuse_what_is_not_on_a_gpu(pkg):
         ch.PagedCache(codes[0], scales, codes, scales)
     with pytest.raises(ex.InvalidArgumentError, match="PagedCache"):
         ch.append(None, x, x, None, None, None)
+
+
+# rows whose column counter would pass 32 bits; operands that only the second of linear's two kernels reads
+def test_refusals_of_the_largest_and_the_misaligned(pkg):
+    lib, big = pkg.lib, 1 << 31
+    assert lib.tfccb200_quantize_tokens_f32(None, P, big, 1, big, P, big, P) == EOVERFLOW
+    for kw in ({"C": P + 2}, {"sb": P + 2}, {"bias": P + 1}):
+        a = dict(stream=None, x=P, ldx=10, B=P, ldb=16, sb=P, bias=None, C=P, M=2, N=10, K=10, act=0, ws=P, ws_len=4096, status=None)
+        a.update(kw)
+        assert lib.tfccb200_qlinear_f32(*a.values()) == EALIGN
+    # 2^24 tiles of 2^23 blocks each
+    s = C.byref(struct(pkg, kv_heads=1, page_size=1024))
+    assert lib.tfccb200_cache_attention_f32(None, s, P, 256, P, 256, P, P, P, 1, 1 << 20, (1 << 29) - 1, 4, (1 << 29) - 1, 1 << 30,
+                                            0.1, 1, P, 1 << 40, None) == EOVERFLOW

@@ -835,7 +835,7 @@ namespace {
 
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
-int run_s8_gemm(const S8GemmArgs& a, int path) {
+int check_s8_gemm(const S8GemmArgs& a) {
   if (!a.A || !a.B || !a.C || !a.a_scales || !a.b_scales || a.M == 0 || a.N == 0 || a.K == 0)
     return TFCCB200_EINVAL;
   if (a.lda < a.K || a.ldb < a.N) return TFCCB200_EINVAL;
@@ -844,6 +844,12 @@ int run_s8_gemm(const S8GemmArgs& a, int path) {
   if (shape_overflows(a.M, a.N, a.K, 1)) return TFCCB200_EOVERFLOW;
   if (misaligned(a.C, 4) || misaligned(a.a_scales, 4) || misaligned(a.b_scales, 4) || misaligned(a.bias, 4))
     return TFCCB200_EALIGN;
+  return TFCCB200_OK;
+}
+
+int run_s8_gemm(const S8GemmArgs& a, int path) {
+  const int st = check_s8_gemm(a);
+  if (st != TFCCB200_OK) return st;
   switch (path) {
     case TFCCB200_PATH_AUTO:
       if (few_s8_gemm_supported(a)) return few_s8_gemm(a);
@@ -896,7 +902,7 @@ int tfccb200_quantize_tokens_f32(void* stream, const float* src, size_t ld_src, 
                                  int8_t* codes, size_t ld_codes, float* scales) {
   if (!src || !codes || !scales || rows == 0 || cols == 0 || ld_src < cols || ld_codes < cols) return TFCCB200_EINVAL;
   if (misaligned(src, 4) || misaligned(scales, 4)) return TFCCB200_EALIGN;
-  if (rows > 0x7fffffffu) return TFCCB200_EOVERFLOW;
+  if (rows > 0x7fffffffu || cols > 0x7fffffffu) return TFCCB200_EOVERFLOW;
   return quantize_tokens(static_cast<cudaStream_t>(stream), src, ld_src, rows, cols, codes, ld_codes, scales);
 }
 
@@ -934,11 +940,9 @@ int tfccb200_qlinear_f32(void* stream, const float* x, size_t ldx, const int8_t*
   a.M = M; a.N = N; a.K = K;
   a.activation = activation;
   a.status = device_status;
-  // everything run_s8_gemm would refuse is refused before the first launch
-  if (!B || !C || !b_scales || N == 0 || ldb < N) return TFCCB200_EINVAL;
-  if (activation != TFCCB200_ACT_NONE && activation != TFCCB200_ACT_GELU_ERF) return TFCCB200_EINVAL;
-  if (K > 133000u || shape_overflows(M, N, K, 1)) return TFCCB200_EOVERFLOW;
-  const int st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
+  int st = check_s8_gemm(a);  // what the product would refuse is refused before the first launch
+  if (st != TFCCB200_OK) return st;
+  st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
   a.early_weights = true;
   return st != TFCCB200_OK ? st : run_s8_gemm(a, TFCCB200_PATH_AUTO);
 }
@@ -992,6 +996,10 @@ int tfccb200_cache_attention_f32(void* stream, const tfccb200_cache* cache, cons
   a.max_new = max_new; a.max_length = max_length;
   a.scale = scale;
   a.causal = causal ? 1 : 0;
+  // the kernels count a kv head's blocks of one sequence in 32 bits
+  const unsigned long long head_rows = static_cast<unsigned long long>(std::min(max_new, rows)) * (heads / a.cache.kv_heads);
+  const unsigned long long length = std::min<unsigned long long>(max_length, static_cast<unsigned long long>(table_width) * a.cache.page_size);
+  if ((head_rows / 128 + 1) * (length / 128 + 4) > 0xffffffffull) return TFCCB200_EOVERFLOW;
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;
   const size_t need = cache_attention_workspace(a);
   if (need && (!workspace || misaligned(workspace, 256) || workspace_bytes < need)) return TFCCB200_EWORKSPACE;
