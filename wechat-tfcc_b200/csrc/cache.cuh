@@ -63,10 +63,18 @@ __device__ __forceinline__ void check_all_sequences(const CacheParams& p) {
     for (unsigned b = threadIdx.x; b < p.batch; b += blockDim.x) load_sequence(p, b);
 }
 
-// Page of position `pos` (< length <= table_width * page_size) of sequence b, or -1.
+// Page of position `pos` (< length <= table_width * page_size) of sequence b, as it stands in the table, and
+// whether there is such a page.
+__device__ __forceinline__ int page_entry(const CacheParams& p, unsigned b, unsigned pos) {
+  return p.table[static_cast<size_t>(b) * p.table_width + (pos >> p.page_shift)];
+}
+__device__ __forceinline__ bool page_exists(const CacheParams& p, int page) {
+  return page >= 0 && static_cast<unsigned>(page) < p.pages;
+}
+// The same at once: -1 (and a report) where there is none.
 __device__ __forceinline__ int page_of(const CacheParams& p, unsigned b, unsigned pos) {
-  const int page = p.table[static_cast<size_t>(b) * p.table_width + (pos >> p.page_shift)];
-  if (page < 0 || static_cast<unsigned>(page) >= p.pages) {
+  const int page = page_entry(p, b, pos);
+  if (!page_exists(p, page)) {
     raise_status(p.status, TFCCB200_DEV_BAD_PAGE);
     return -1;
   }

@@ -262,20 +262,29 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           const uint32_t s = n & 1u;
           float ks[4], vs[4];
           uint32_t top = __float_as_uint(kValueFloor);
+          // (pages first, then all scales, reports last: a report between two loads would order them)
+          int page[4];
+          bool bad = false;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int pos = static_cast<int>(blk * kBlockKeys + i * 32 + lane);
-            ks[i] = vs[i] = 0.f;
-            if (pos < it.length) {
-              const int page = page_of(a.c, it.b, pos);
-              if (page >= 0) {
-                const size_t at = cache_slot(a.c, page, it.head, pos);
-                ks[i] = a.c.key_scales[at];
-                vs[i] = a.c.value_scales[at];
-              } else {  // a page that does not exist shows as NaN
-                ks[i] = vs[i] = __uint_as_float(0x7fffffffu);
-              }
+            page[i] = pos < it.length ? page_entry(a.c, it.b, pos) : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int pos = static_cast<int>(blk * kBlockKeys + i * 32 + lane);
+            const bool real = page_exists(a.c, page[i]);
+            bad |= !real;
+            ks[i] = vs[i] = real ? 0.f : __uint_as_float(0x7fffffffu);  // a page that does not exist shows as NaN
+            if (pos < it.length && real) {
+              const size_t at = cache_slot(a.c, page[i], it.head, pos);
+              ks[i] = a.c.key_scales[at];
+              vs[i] = a.c.value_scales[at];
             }
+          }
+          if (bad) raise_status(a.c.status, TFCCB200_DEV_BAD_PAGE);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
             const uint32_t bits = __float_as_uint(vs[i]) & 0x7fffffffu;
             if (bits < 0x7f800000u) top = max(top, bits);
           }
