@@ -39,8 +39,8 @@ namespace {
 //   Output: V becomes fp16 (1.5 instructions a code), weights as above; with 8 rows the 16 rows of
 //   m16n8k16 hold their hi and lo terms side by side.
 // Eight warps take the eight 16-key groups of a 128-key block and are added at the item's end.
-// Two sequences of 65536 keys, 64 / 8 heads of 128: 68 us, 4.06 TB/s, 0.62 of the measured copy rate; 32 ragged
-// ones, 32 / 8 heads: 75 us.  Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is
+// Two sequences of 65536 keys, 64 / 8 heads of 128: 69 us, 4.0 TB/s, 0.61 of the measured copy rate; 32 ragged
+// ones, 32 / 8 heads: 74 us.  Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is
 // left is 4 us until the first loads, CTAs that finish 10 us apart, 4 us per item of a short sequence,
 // and the merge.  (Scores from fp16 terms of q instead of digits 83 us; three CTAs per SM with 80 registers
 // 126 us, because of spills.)
