@@ -144,6 +144,9 @@ def launch_count() -> int:
     return int(lib.tfccb200_launch_count())
 
 
+EWORKSPACE = -3  # TFCCB200_EWORKSPACE
+
+
 def check(status: int) -> None:
     """Turn a C-ABI status into the matching exception."""
     if status == 0:

@@ -22,7 +22,7 @@ import ctypes as C
 import torch
 
 from . import exceptions
-from ._lib import check, lib
+from ._lib import EWORKSPACE, check, lib
 from .session import launch_context
 
 
@@ -79,15 +79,16 @@ def _sequences(cache, starts, lengths, table):
     """(starts, lengths, table pointers, batch, table width) of a call, checked."""
     if not isinstance(cache, PagedCache):
         raise exceptions.InvalidArgumentError("cache must be a PagedCache")
-    device = cache.device
+    index = cache.device.index
     for t, name, rank in ((starts, "starts", 1), (lengths, "lengths", 1), (table, "table", 2)):
-        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != rank or t.numel() == 0 or \
-                not t.is_cuda or t.get_device() != device.index or not t.is_contiguous():
+        # (a tensor of the CPU has device -1)
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != index or \
+                len(t.shape) != rank or 0 in t.shape or not t.is_contiguous():
             raise exceptions.InvalidArgumentError(f"{name}: expected a contiguous int32 tensor of rank {rank} on {cache.device}")
-    batch = lengths.shape[0]
-    if starts.shape[0] != batch + 1 or table.shape[0] != batch:
+    batch, width = table.shape
+    if lengths.shape[0] != batch or starts.shape[0] != batch + 1:
         raise exceptions.InvalidArgumentError("starts, lengths and table don't match")
-    return starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), batch, table.shape[1]
+    return starts.data_ptr(), lengths.data_ptr(), table.data_ptr(), batch, width
 
 
 def _packed(t, name, rows, width, device):
@@ -98,7 +99,7 @@ def _packed(t, name, rows, width, device):
     if t.dtype is not torch.float32:
         raise exceptions.NotImplementedError(f"{name}: implemented for float32, got {t.dtype}")
     pitch, step = t.stride()
-    if not t.is_cuda or t.get_device() != device.index or step != 1:
+    if t.get_device() != device.index or step != 1:
         raise exceptions.InvalidArgumentError(f"{name}: rows must be contiguous, on {device}")
     return width if shape[0] == 1 else pitch
 
@@ -174,9 +175,12 @@ def attention(cache: PagedCache, q: torch.Tensor, starts: torch.Tensor, lengths:
         scale = 1.0 / float(cache.dim) ** 0.5
     sess, stream, guard = launch_context(cache.device)
     with guard:
-        ws_ptr, ws_len, _owner = sess.workspace_on(
-            lib.tfccb200_cache_attention_workspace(cache._ref, batch, rows, heads, max_new, max_length), stream)
-        check(lib.tfccb200_cache_attention_f32(stream, cache._ref, q.data_ptr(), ldq, out.data_ptr(),
-                                               ldo, ps, pl, pt, batch, width, rows, heads, max_new, max_length,
-                                               float(scale), 1 if causal else 0, ws_ptr, ws_len, sess.status_ptr))
+        args = (stream, cache._ref, q.data_ptr(), ldq, out.data_ptr(), ldo, ps, pl, pt, batch, width, rows, heads,
+                max_new, max_length, float(scale), 1 if causal else 0)
+        st = lib.tfccb200_cache_attention_f32(*args, *sess.scratch_on(stream), sess.status_ptr)
+        if st == EWORKSPACE:  # (refused before any launch)
+            need = lib.tfccb200_cache_attention_workspace(cache._ref, batch, rows, heads, max_new, max_length)
+            ws_ptr, ws_len, _owner = sess.workspace_on(need)
+            st = lib.tfccb200_cache_attention_f32(*args, ws_ptr, ws_len, sess.status_ptr)
+        check(st)
     return out

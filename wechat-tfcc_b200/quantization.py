@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 
 from . import exceptions
-from ._lib import ACTIVATIONS, PATHS, check, lib
+from ._lib import ACTIVATIONS, EWORKSPACE, PATHS, check, lib
 from .session import get_session, launch_context
 
 _REDUCE = {torch.uint8: "tfccb200_reduce_sum_u8", torch.int8: "tfccb200_reduce_sum_s8",
@@ -377,8 +377,10 @@ def linear(x: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch
     out = x.new_empty(x.shape[:-1] + (n,))
     sess, stream, guard = launch_context(x.device)
     with guard:
-        ws_ptr, ws_len, _owner = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k), stream)
-        check(lib.tfccb200_qlinear_f32(stream, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias,
-                                       out.data_ptr(), m, n, k, ACTIVATIONS[activation], ws_ptr, ws_len,
-                                       sess.status_ptr))
+        args = (stream, x.data_ptr(), ldx, b.data_ptr(), ldb, sb, sbias, out.data_ptr(), m, n, k, ACTIVATIONS[activation])
+        st = lib.tfccb200_qlinear_f32(*args, *sess.scratch_on(stream), sess.status_ptr)
+        if st == EWORKSPACE:  # (refused before any launch)
+            ws_ptr, ws_len, _owner = sess.workspace_on(lib.tfccb200_qlinear_workspace(m, k))
+            st = lib.tfccb200_qlinear_f32(*args, ws_ptr, ws_len, sess.status_ptr)
+        check(st)
     return out

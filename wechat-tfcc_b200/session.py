@@ -33,19 +33,21 @@ class Session:
     def status_ptr(self) -> int:
         return self._status.data_ptr()
 
-    def workspace_on(self, nbytes: int, stream_ptr: int):
-        """``(pointer, bytes, owner)`` of scratch for one call on the current stream, whose handle the
-        caller already has: the stream's buffer (:meth:`workspace`), or under capture one of the call's own, so
-        that captured graphs, which may be replayed side by side, share none.  ``owner`` has to live
-        until the call is launched."""
-        if nbytes == 0:
-            return None, 0, None
-        if _capturing():
+    def scratch_on(self, stream_ptr: int):
+        """``(pointer, bytes)`` of the current stream's buffer as it stands, to offer to an entry point that
+        checks what it needs before it launches anything; nothing under capture, see :meth:`workspace_on`."""
+        ws = self._workspaces.get(stream_ptr)
+        if ws is None or _capturing():
+            return None, 0
+        return ws.data_ptr(), ws.numel()
+
+    def workspace_on(self, nbytes: int):
+        """``(pointer, bytes, owner)`` of scratch for one call on the current stream: the stream's buffer
+        (:meth:`workspace`), or under capture one of the call's own, so that captured graphs, which may
+        be replayed side by side, share none.  ``owner`` has to live until the call is launched."""
+        if nbytes and _capturing():
             own = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             return own.data_ptr(), nbytes, own
-        ws = self._workspaces.get(stream_ptr)
-        if ws is not None and ws.numel() >= nbytes:
-            return ws.data_ptr(), ws.numel(), ws
         return *self.workspace(nbytes), None
 
     def workspace(self, nbytes: int):
