@@ -382,10 +382,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (kMask) vscale[j] = key0 + (j & 1) + (j >> 1) * 8 < length ? vscale[j] : 0.f;
-        grows |= vscale[j] > vref;
+        grows |= fabsf(vscale[j]) > vref;
       }
       if (__any_sync(0xffffffffu, grows)) {
-        float vmax = fmaxf(fmaxf(vscale[0], vscale[1]), fmaxf(vscale[2], vscale[3]));
+        float vmax = fmaxf(fmaxf(fabsf(vscale[0]), fabsf(vscale[1])), fmaxf(fabsf(vscale[2]), fabsf(vscale[3])));
         vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
         vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
         float vnext = vref;  // largest value scale so far, rounded up to a power of two
