@@ -73,3 +73,78 @@ def test_scales_of_either_sign(pkg, new, dim, share):
         t[torch.rand(t.shape, device=dev(), generator=s.g) < share] *= -1
     want, tol = exact(s, q, 8, 1 / math.sqrt(dim))
     compare(run(s, q, None), want, tol, new)
+
+
+# ---- value scales ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("power", [12, 20, 40, 66, 120])
+@pytest.mark.parametrize("new,heads,kv,dim", [(8, 1, 1, 128), (8, 4, 2, 64), (5, 2, 1, 128), (200, 4, 2, 128), (200, 2, 2, 64), (3, 40, 1, 128)])
+def test_a_token_that_a_row_does_not_see_leaves_its_result_alone(pkg, new, heads, kv, dim, power):
+    """The value scales of later new tokens are 2^power times the others."""
+    n = 330
+    s = Setup(pkg, [new], [n], kv, dim, 16, seed=power + new)
+    q = torch.randn(new, heads * dim, device=dev(), generator=s.g)
+    page, slot = s.where(0)
+    for back in {1, max(1, new // 2)}:  # tokens n - back .. n - 1
+        s.cache.value_scales[page[n - back], :, slot[n - back]] *= 2.0 ** power
+    want, tol = exact(s, q, heads, 1 / math.sqrt(dim))
+    compare(run(s, q, None), want, tol, new)
+
+
+@pytest.mark.parametrize("value", [math.inf, 3e38])
+@pytest.mark.parametrize("new", [8, 200])
+def test_the_largest_and_infinite_scales_stay_with_the_rows_that_see_them(pkg, new, value):
+    n, dim = 330, 128
+    s = Setup(pkg, [new], [n], 1, dim, 64, seed=new)
+    q = torch.randn(new, 2 * dim, device=dev(), generator=s.g)
+    want, tol = exact(s, q, 2, 1 / math.sqrt(dim))
+    page, slot = s.where(0)
+    bad = n - new // 2
+    s.cache.value_scales[page[bad], 0, slot[bad]] = value
+    compare(run(s, q, None), want, tol, bad - (n - new))
+
+
+@pytest.mark.parametrize("power,below", [(20, 127), (40, 127), (30, 21), (12, 9), (66, 40), (100, 75)])
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 4, 1, 128), (1, 16, 2, 64), (8, 2, 2, 128), (16, 2, 2, 64), (200, 2, 1, 64), (150, 2, 2, 128)])
+def test_a_token_of_small_weight_and_large_values(pkg, new, heads, kv, dim, power, below):
+    """Tokens that every row sees with a score `below` under the others (in natural units, about) and value scales
+    2^power times theirs: from no share in the result to most of it.  They lie in the first block, in the middle
+    and in the last."""
+    n = 700
+    s = Setup(pkg, [new], [n], kv, dim, 32, seed=power + new + dim)
+    q = torch.randn(new, heads * dim, device=dev(), generator=s.g)
+    q.view(new, heads, dim)[:, :, 0] = 8.0
+    page, slot = s.where(0)
+    for pos in (5, 300, n - new):
+        s.cache.keys[page[pos], :, slot[pos]] = 0
+        s.cache.keys[page[pos], :, slot[pos], 0] = -127
+        s.cache.key_scales[page[pos], :, slot[pos]] = below / 127
+        s.cache.value_scales[page[pos], :, slot[pos]] *= 2.0 ** power
+    want, tol = exact(s, q, heads, 0.125)
+    compare(run(s, q, 0.125), want, tol, new)
+
+
+@pytest.mark.parametrize("new", [1, 8, 200])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_value_scales_spread_over_many_powers(pkg, new, dim):
+    """No two tokens alike: scales over 60 powers of two in three sequences, one of them within one page, and zero
+    scales among them."""
+    s = Setup(pkg, [new, new, new], [700, 300, new + 3], 2, dim, 16, seed=new)
+    q = torch.randn(s.rows, 4 * dim, device=dev(), generator=s.g)
+    s.cache.value_scales *= torch.exp2(torch.randint(-30, 31, s.cache.value_scales.shape, device=dev(), generator=s.g).float())
+    s.cache.value_scales[torch.rand(s.cache.value_scales.shape, device=dev(), generator=s.g) < 0.1] = 0.0
+    want, tol = exact(s, q, 4, 1 / math.sqrt(dim))
+    compare(run(s, q, None), want, tol, s.rows)
+
+
+@pytest.mark.parametrize("news,lengths", [([1, 1], [9000, 5000]), ([160], [6000])])
+def test_pieces_of_cut_items_with_scales_that_differ(pkg, news, lengths):
+    """Long sequences, whose keys several CTAs share: each piece has a range of scales of its own."""
+    s = Setup(pkg, news, lengths, 1, 128, 64, seed=3)
+    q = torch.randn(s.rows, 2 * 128, device=dev(), generator=s.g)
+    page, slot = s.where(0)
+    step = torch.arange(len(page), device=dev()) // 1000
+    s.cache.value_scales[page, 0, slot] *= torch.exp2(10.0 * step)
+    want, tol = exact(s, q, 2, 1 / math.sqrt(128))
+    compare(run(s, q, None), want, tol, s.rows)

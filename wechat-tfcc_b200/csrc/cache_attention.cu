@@ -8,7 +8,9 @@
 //
 // The weights w_j = p_j vs_j carry the value scales.  Codes are exact in fp16, and a weight is split into
 // two fp16 terms, w = hi + lo with 11 bits each, after scaling by a power of two that bounds the
-// weights; two products with fp32 sums then give 22 bits where one would give 11.  The softmax is
+// weights; two products with fp32 sums then give 22 bits where one would give 11.  That power is taken
+// per row from the keys the row sees, w_j among them and not vs_j alone: a token that is hidden from a row, or
+// has next to no weight in it, takes no bits from the others however large its values are.  The softmax is
 // the one-pass form: a reference maximum and a sum in fp32, sums rescaled when a score exceeds the
 // reference by more than kLazy (in log2 units), which is rare after the first keys.
 #include <cuda_runtime.h>
@@ -55,7 +57,7 @@ struct FewLayout {
   static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
   static constexpr int kFragBytes = (DIM / 32) * 32 * (ROWS == 8 ? 16 + 8 : 3 * 16);  // digits of q
   static constexpr int kSmall = kFragBytes + kFewWarps * kRingBytes;
-  static constexpr int kSmem = kSmall + (kFewWarps * 2 * ROWS + kFewWarps) * 4;
+  static constexpr int kSmem = kSmall + kFewWarps * 3 * ROWS * 4;
   static_assert(ROWS * DIM * 4 <= kRingBytes, "a warp's sums reuse its ring");
 };
 
@@ -122,8 +124,13 @@ __device__ __forceinline__ unsigned value_chunk(unsigned r, unsigned c) {
   else return (r >> 1) * 128 + (((((r & 1u) << 2) + c) ^ (r & 6u)) << 4);
 }
 
-constexpr float kWeightTop = 1024.f;           // weights are scaled to at most 2^10, times 2^kLazy: fp16
-constexpr float kLazy = 5.f;                   // keeps 22 bits of them down to 2^-13 of the top
+// The unit of a row's weights: the value scale `vref`, a power of two, is held as kWeightTop = 2^10, so that weights
+// reach at most 2^10 2^kLazy, inside fp16's range, and have 22 bits down to 2^-13 of the top.  vref is the largest
+// scale that the row has met, but at most kValueRange times its largest weight so far (p_j vs_j, with p_j = 1 at
+// the reference maximum): a weight's absolute error is then at most 2^-25 2^-10 vref <= 2^-26 of the largest weight.
+constexpr float kWeightTop = 1024.f;
+constexpr float kLazy = 5.f;
+constexpr float kValueRange = 512.f;
 constexpr float kValueFloor = 7.8886091e-31f;  // 2^-100
 
 template <int DIM, int ROWS>
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
   const uint32_t ring_addr = ptx::smem_u32(ring);
   float* red_m = reinterpret_cast<float*>(smem + L::kSmall);  // [warp][row]
   float* red_l = red_m + kFewWarps * ROWS;
-  float* red_v = red_l + kFewWarps * ROWS;  // [warp]
+  float* red_v = red_l + kFewWarps * ROWS;
 
   ThreadSequence mine;
   const unsigned long long units = all_units<ROWS, kFewThreads>(a, &sched, &mine);
@@ -291,9 +298,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int j = 0; j < ROWS / 4; ++j) o[i][j] = 0.f;
-    float top[ROWS / 8], sum[ROWS / 8], vref = kValueFloor, vup = kWeightTop / kValueFloor;
+    float top[ROWS / 8], sum[ROWS / 8], vup[ROWS / 8];  // vup = kWeightTop / vref
 #pragma unroll
-    for (int h = 0; h < ROWS / 8; ++h) top[h] = -INFINITY, sum[h] = 0.f;
+    for (int h = 0; h < ROWS / 8; ++h) top[h] = -INFINITY, sum[h] = 0.f, vup[h] = kWeightTop / kValueFloor;
 
     int st = 0;
     // keys below this are seen by every row of the item
@@ -367,51 +374,68 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       const float2 va = *reinterpret_cast<const float2*>(ks + 16 + 2 * t), vb = *reinterpret_cast<const float2*>(ks + 24 + 2 * t);
       const int key0 = static_cast<int>(blk * kBlockKeys + warp * 16 + 2 * t);
       const float kscale[4] = {ka.x, ka.y, kb.x, kb.y};
-      float vscale[4] = {va.x, va.y, vb.x, vb.y};
+      const float vscale[4] = {va.x, va.y, vb.x, vb.y};
+      auto seen = [&](int h, int j) { return !kMask || key0 + (j & 1) + (j >> 1) * 8 < sees[h]; };
+      float vs[ROWS / 8][4];  // value scales in the row's unit, 0 where it does not see the key
+      auto scale_values = [&](int h) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[h][j] = seen(h, j) ? vscale[j] * vup[h] : 0.f;
+      };
       bool grows = false;
 #pragma unroll
       for (int h = 0; h < ROWS / 8; ++h) {
         const float limit = top[h] + kLazy;  // -inf before the first key
+        scale_values(h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[h][j] *= kscale[j] * row_scale[h];
-          if constexpr (kMask) x[h][j] = key0 + (j & 1) + (j >> 1) * 8 < sees[h] ? x[h][j] : -INFINITY;
+          if constexpr (kMask) x[h][j] = seen(h, j) ? x[h][j] : -INFINITY;
           grows |= x[h][j] > limit;
+          grows |= fabsf(vs[h][j]) > kWeightTop;
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kMask) vscale[j] = key0 + (j & 1) + (j >> 1) * 8 < length ? vscale[j] : 0.f;
-        grows |= fabsf(vscale[j]) > vref;
-      }
       if (__any_sync(0xffffffffu, grows)) {
-        float vmax = fmaxf(fmaxf(fabsf(vscale[0]), fabsf(vscale[1])), fmaxf(fabsf(vscale[2]), fabsf(vscale[3])));
-        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-        float vnext = vref;  // largest value scale so far, rounded up to a power of two
-        if (vmax > vref) vnext = __uint_as_float(min((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
-        const float vf = vref / vnext;
-        vref = vnext;
-        vup = kWeightTop / vref;
 #pragma unroll
         for (int h = 0; h < ROWS / 8; ++h) {
           float m = fmaxf(fmaxf(x[h][0], x[h][1]), fmaxf(x[h][2], x[h][3]));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
           const float next = m > top[h] + kLazy ? m : top[h];
-          const float f = exp2_fast(top[h] - (next == -INFINITY ? 0.f : next));
+          const float ref = next == -INFINITY ? 0.f : next;
+          const float f = exp2_fast(top[h] - ref);
+          const float vref = kWeightTop / vup[h];
+          float v = vref, w = f * (vref * (1.f / kValueRange));  // (the largest weight so far is no smaller)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float y = seen(h, j) ? fabsf(vscale[j]) : 0.f;
+            v = fmaxf(v, y);
+            w = fmaxf(w, exp2_fast(x[h][j] - ref) * y);
+          }
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
+          // powers of two: v upwards, the bound on it downwards
+          v = __uint_as_float(min((__float_as_uint(v) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
+          v = fmaxf(fminf(v, __uint_as_float(__float_as_uint(w * kValueRange) & 0x7f800000u)), kValueFloor);
+          const float up = kWeightTop / v;
+          // (f = 0: nothing so far counts, and up / vup may be infinite)
+          const float fv = f == 0.f ? 0.f : f * (up / vup[h]);
           sum[h] *= f;
           top[h] = next;
+          vup[h] = up;
+          scale_values(h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // (a finite scale of a weight that underflows stays finite: 0 * inf)
+            if (fabsf(vscale[j]) < INFINITY) vs[h][j] = fminf(fmaxf(vs[h][j], -3.4e38f), 3.4e38f);
 #pragma unroll
           for (int i = 0; i < kTiles; ++i) {
-            o[i][2 * h] *= f * vf;
-            o[i][2 * h + 1] *= f * vf;
+            o[i][2 * h] *= fv;
+            o[i][2 * h + 1] *= fv;
           }
         }
       }
       uint32_t hi[ROWS / 8][2], lo[ROWS / 8][2];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vscale[j] *= vup;
 #pragma unroll
       for (int h = 0; h < ROWS / 8; ++h) {
         const float base = top[h] == -INFINITY ? 0.f : top[h];
@@ -420,9 +444,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
         for (int j = 0; j < 4; ++j) {
           const float p = exp2_fast(x[h][j] - base);
           sum[h] += p;
-          w[j] = p * vscale[j];
-          if constexpr (kMask)  // (0 * NaN)
-            w[j] = key0 + (j & 1) + (j >> 1) * 8 < sees[h] ? w[j] : 0.f;
+          w[j] = p * vs[h][j];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -493,9 +515,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       if (t == 0) {
         red_m[warp * ROWS + g + 8 * h] = top[h];
         red_l[warp * ROWS + g + 8 * h] = sum[h];
+        red_v[warp * ROWS + g + 8 * h] = 1.f / vup[h];
       }
     }
-    if (lane == 0) red_v[warp] = vref;
     __syncwarp();
     {
       float* dst = reinterpret_cast<float*>(ring);
@@ -529,7 +551,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       for (int w = 0; w < kFewWarps; ++w) {
         const float f = exp2_fast(red_m[w * ROWS + r] - base);
         l += f * red_l[w * ROWS + r];
-        const float fv = f * (red_v[w] * (1.f / kWeightTop));
+        const float fv = f * red_v[w * ROWS + r];
         const float4 y = *reinterpret_cast<const float4*>(smem + L::kFragBytes + w * L::kRingBytes + (r * DIM + d) * 4);
         acc.x += fv * y.x; acc.y += fv * y.y; acc.z += fv * y.z; acc.w += fv * y.w;
       }

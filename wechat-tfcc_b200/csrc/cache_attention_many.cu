@@ -5,9 +5,9 @@
 // q per row after scaling by a power of two, and the weights w_j = p_j vs_j as in
 // cache_attention.cu.  Per block
 //   S = Q_hi K^T + Q_lo K^T          A from tensor memory, K from shared memory, fp32 sums
-//   P = exp2(S ks - m) vs            hi and lo terms go back over S
+//   P = exp2(S ks - r) vs            r: the row's largest score in the block; hi and lo terms go back over S
 //   O_block = P_hi V + P_lo V        A from tensor memory, V as it lies (MN-major)
-//   O = O alpha + O_block            fp32 registers
+//   O = O alpha + 2^(r - m) O_block  fp32 registers, m the row's running maximum
 // The tensor core's accumulator narrows without rounding to nearest, which would bias O over
 // thousands of keys; summed from zero per block and added to registers it does not, and a block's
 // own power of two for the value scales comes along for nothing.
@@ -31,7 +31,9 @@
 // measured on the way there (the same case): a thread per row with all of its 128 sums, two
 // tiles per CTA 1137; two threads per row 1193; this layout 955; products issued with precomputed
 // descriptors 932; items weighted in the schedule 870; scales in the order of their reading 838.
-// Ordinary loads in place of read-only ones, pages looked up four at a time: 840.
+// Ordinary loads in place of read-only ones, pages looked up four at a time: 840.  References per block
+// and the path for value scales that spread wide: 833 to 844 (with that path in the registers of the main one 850 to
+// 885).
 // Slower: sixteen softmax warps 1088, products summed over four blocks in tensor memory 972, codes
 // through a ring of bulk copies 880, code loads two tiles ahead 930,
 // the next tile's loads between this one's stores 995.
@@ -55,7 +57,15 @@ constexpr int kTileBytes = 128 * 128;  // 128 rows x 64 fp16, 128-byte swizzle
 constexpr int kRegsControl = 48, kRegsConvert = 96, kRegsSoftmax = 184;
 static_assert(kRegsControl + kRegsConvert + 2 * kRegsSoftmax == 512, "shares of 128 registers per thread at launch");
 
-constexpr float kWeightTop = 1024.f;  // weights reach at most 2^10 times 2^kLazy, inside fp16's range
+// The unit of a block's weights: its largest value scale, rounded up to a power of two E, is held as kWeightTop
+// = 2^14, and a row's exponentials are taken relative to its own largest score in the block, so that
+// weights reach at most 2^14.  As long as the block's scales lie within 2^kValueRange of E, the row's largest weight
+// is no less than 2^(14 - kValueRange), and fp16's absolute error of 2^-25 is 2^-30 of it.  Where they spread
+// wider, in keys that the row may not even see, the unit is a row's own largest weight instead (wide_block).
+constexpr float kWeightTop = 16384.f;
+constexpr int kValueRange = 9;
+constexpr uint32_t kWideTop = 0x71800000u;     // 2^100
+constexpr float kWideUnit = 1.0995116e12f;     // 2^40
 constexpr float kLazy = 5.f;          // the maximum moves only when it grows by more (log2 units)
 constexpr float kValueFloor = 7.8886091e-31f;  // 2^-100
 
@@ -89,6 +99,14 @@ struct ManyLayout {
   static constexpr int kTmemQ = 0, kTmemS = 128, kTmemO = 384;  // columns
   static_assert(kSmem <= 232448, "shared memory");
 };
+
+// 2^(x - m), 0 for x = -inf whatever m is.
+__device__ __forceinline__ float relative_to(float x, float m) { return x == -INFINITY ? 0.f : exp2_fast(x - m); }
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 struct Waiter {
   volatile uint32_t* abort_flag;
@@ -135,7 +153,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
   static_assert(14 + 2 * L::kRing <= L::kNumBars, "barriers");
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem + L::kMisc);
   volatile uint32_t* abort_flag = misc + 1;
-  volatile float* value_back = reinterpret_cast<volatile float*>(misc + 2);  // per scale stage
+  volatile float* value_back = reinterpret_cast<volatile float*>(misc + 2);  // per scale stage: value of the scales' unit, negative where they spread wide
   const Item* items = reinterpret_cast<const Item*>(smem + L::kItems);
   ScheduleShared* sched = reinterpret_cast<ScheduleShared*>(smem + L::kSched);
   const Waiter wait{abort_flag, a.c.status, timeout_ns};
@@ -292,7 +310,14 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           }
           top = __reduce_max_sync(0xffffffffu, top);
           top = min((top + 0x7fffffu) & 0x7f800000u, 0x7f000000u);  // up to a power of two
-          const float up = kWeightTop / __uint_as_float(top);
+          bool wide = false;  // a scale other than 0 lies 2^kValueRange below
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            wide |= (__float_as_uint(vs[i]) & 0x7fffffffu) - 1u < top - (static_cast<uint32_t>(kValueRange) << 23) - 1u;
+          wide = __any_sync(0xffffffffu, wide);
+          // wide: scales as they are, or brought down so that exponentials relative to a weight have the range for it
+          const float unit = !wide ? __uint_as_float(top) * (1.f / kWeightTop) : top > kWideTop ? kWideUnit : 1.f;
+          const float up = 1.f / unit;
           if (!wait(sc_empty + 8 * s, ((n >> 1) & 1u) ^ 1u, TFCCB200_DEV_TIMEOUT_CONVERT)) return false;
           float* dst = reinterpret_cast<float*>(smem + L::kScales + s * L::kScaleBytes);
 #pragma unroll
@@ -301,7 +326,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
             dst[at] = ks[i];
             dst[4 * kScalePitch + at] = vs[i] * up;
           }
-          if (lane == 0) value_back[s] = __uint_as_float(top) * (1.f / kWeightTop);
+          if (lane == 0) value_back[s] = wide ? -unit : unit;
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(sc_full + 8 * s);
         }
@@ -495,7 +520,6 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         // scales of this thread's keys 8 i + 2 t, + 1 for two i at a time, then of their values
         const ulonglong2* ks_at = reinterpret_cast<const ulonglong2*>(smem + L::kScales + s * L::kScaleBytes) + t * (kScalePitch / 4);
         const ulonglong2* vs_at = ks_at + kScalePitch;
-        if (!wait(sc_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         if (!wait(s_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
         ptx::tc_fence_after_sync();
         const int first = static_cast<int>((it.lo + j) * kBlockKeys + 2 * t);  // the thread's first key
@@ -521,6 +545,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
             top[k] = fmaxf(top[k], fmaxf(u.x, u.y));
           }
         }
+        const uint64_t rs2[2] = {pair(rs[0], rs[0]), pair(rs[1], rs[1])};
         bool grows = false;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -532,7 +557,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const float next = top[k] > m[k] + kLazy ? top[k] : m[k];
-            const float f = exp2_fast(m[k] - (next == -INFINITY ? 0.f : next));
+            const float f = relative_to(m[k], next);
             m[k] = next;
             l[k] *= f;
             back[k] *= f;
@@ -545,8 +570,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         }
         // -- weights, as two terms over the scores they come from: 16 scores become 8 columns of hi
         // and 8 of lo terms --
-        const uint64_t rs2[2] = {pair(rs[0], rs[0]), pair(rs[1], rs[1])};
-        const float r0 = m[0] == -INFINITY ? 0.f : -m[0], r1 = m[1] == -INFINITY ? 0.f : -m[1];
+        const float r0 = top[0] == -INFINITY ? 0.f : -top[0], r1 = top[1] == -INFINITY ? 0.f : -top[1];
         const uint64_t ref2[2] = {pair(r0, r0), pair(r1, r1)};
         uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
@@ -577,10 +601,12 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float2 f = unpair(l2[k]);
-          l[k] += f.x + f.y;
+          top[k] = relative_to(top[k], m[k]);
+          l[k] = fmaf(f.x + f.y, top[k], l[k]);
         }
         if (j && !drain(nb - 1)) return false;
-        back[0] = back[1] = value_back[s];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) back[k] = value_back[s] * top[k];
         ptx::tmem_st_wait();
         ptx::tc_fence_before_sync();
         __syncwarp();
@@ -590,7 +616,119 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         }
         return true;
       };
+      // One block whose value scales spread wide.  A row's reference is the one that puts its largest weight at
+      // 2^13 (but no less than 2^-60 of its largest exponential, for the sum of these).  The scores are
+      // read from tensor memory twice, 64 at a time: kept, they would cost the loop above registers.
+      auto wide_block = [&](unsigned j) {
+        const unsigned s = nb & 1u;
+        const uint32_t t_s = rows_addr + L::kTmemS + s * 128;
+        const float2* const ks_at = reinterpret_cast<const float2*>(smem + L::kScales + s * L::kScaleBytes) + t * (kScalePitch / 2);
+        const float2* const vs_at = ks_at + 2 * kScalePitch;
+        if (!wait(s_full + 8 * s, (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
+        ptx::tc_fence_after_sync();
+        const int first = static_cast<int>((it.lo + j) * kBlockKeys + 2 * t);
+        float ref[2] = {-INFINITY, -INFINITY}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        // scores 64 h .. of the block, -inf where a row does not see the key
+        auto scores = [&](int h, uint32_t (&x)[32]) {
+          ptx::tmem_ld_16x64(t_s + 64 * h, x);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 ks = ks_at[8 * h + i];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t* const e = &x[4 * i + 2 * k];
+              const int key = first + 64 * h + 8 * i;
+              e[0] = __float_as_uint(key < sees[k] ? __uint_as_float(e[0]) * ks.x * rs[k] : -INFINITY);
+              e[1] = __float_as_uint(key + 1 < sees[k] ? __uint_as_float(e[1]) * ks.y * rs[k] : -INFINITY);
+            }
+          }
+        };
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[32];
+          scores(h, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 vs = vs_at[8 * h + i];
+            const float lx = fabsf(vs.x) < INFINITY ? log2_fast(fabsf(vs.x)) : -INFINITY;
+            const float ly = fabsf(vs.y) < INFINITY ? log2_fast(fabsf(vs.y)) : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // (the maxima pass over NaN)
+              const float u = __uint_as_float(x[4 * i + 2 * k]), v = __uint_as_float(x[4 * i + 2 * k + 1]);
+              top[k] = fmaxf(top[k], fmaxf(u, v));
+              ref[k] = fmaxf(ref[k], fmaxf(u + lx, v + ly));
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int o2 = 1; o2 < 4; o2 <<= 1) {
+            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o2));
+            ref[k] = fmaxf(ref[k], __shfl_xor_sync(0xffffffffu, ref[k], o2));
+          }
+          ref[k] = fmaxf(ref[k] - 13.f, top[k] - 60.f);
+          if (top[k] > m[k] + kLazy) {
+            const float f = relative_to(m[k], top[k]);
+            m[k] = top[k];
+            l[k] *= f;
+            back[k] *= f;
+#pragma unroll
+            for (int i = 0; i < DIM / 8; ++i) {
+              o[4 * i + 2 * k] *= f;
+              o[4 * i + 2 * k + 1] *= f;
+            }
+          }
+        }
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[32];
+          scores(h, x);
+#pragma unroll
+          for (int ch = 0; ch < 2; ++ch) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int c = 4 * ch + i, key = first + 64 * h + 8 * c;
+              const float2 vs = vs_at[8 * h + c];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float r = ref[k] == -INFINITY ? 0.f : ref[k];
+                const float px = exp2_fast(__uint_as_float(x[4 * c + 2 * k]) - r), py = exp2_fast(__uint_as_float(x[4 * c + 2 * k + 1]) - r);
+                sum[k] += px + py;
+                const float ux = key < sees[k] ? px * vs.x : 0.f, uy = key + 1 < sees[k] ? py * vs.y : 0.f;
+                const uint32_t hi = pack_half2(ux, uy);
+                w[2 * (4 * (i >> 1) + (i & 1)) + k] = hi;
+                w[2 * (4 * (i >> 1) + 2 + (i & 1)) + k] = pack_rest(ux, uy, hi);
+              }
+            }
+            ptx::tmem_st_16x32(t_s + 64 * h + ch * 32, w);
+          }
+          ptx::tmem_st_wait();
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          ref[k] = relative_to(ref[k], m[k]);
+          l[k] = fmaf(sum[k], ref[k], l[k]);
+        }
+        if (j && !drain(nb - 1)) return false;
+        back[0] = -value_back[s] * ref[0];
+        back[1] = -value_back[s] * ref[1];
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(sc_empty + 8 * s);
+          ptx::mbar_arrive(p_full);
+        }
+        return true;
+      };
       for (unsigned j = 0; j < blocks; ++j, ++nb) {
+        if (!wait(sc_full + 8 * (nb & 1u), (nb >> 1) & 1u, TFCCB200_DEV_TIMEOUT_EPILOGUE)) return false;
+        if (value_back[nb & 1u] < 0.f) {
+          if (!wide_block(j)) return false;
+          continue;
+        }
         const bool masked = static_cast<int>((it.lo + j + 1) * kBlockKeys) > all_see;  // the same in all rows
         if (!(masked ? block(j, std::true_type()) : block(j, std::false_type()))) return false;
       }
