@@ -148,3 +148,23 @@ def test_pieces_of_cut_items_with_scales_that_differ(pkg, news, lengths):
     s.cache.value_scales[page, 0, slot] *= torch.exp2(10.0 * step)
     want, tol = exact(s, q, 2, 1 / math.sqrt(128))
     compare(run(s, q, None), want, tol, s.rows)
+
+
+# ---- q --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("large", [100.0, 1000.0, 16384.0])
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 8, 1, 128), (1, 8, 2, 64), (2, 8, 1, 128), (16, 1, 1, 64), (60, 2, 1, 128), (60, 4, 2, 64)])
+@pytest.mark.parametrize("n", [64, 90])
+def test_an_outlier_channel_of_q_on_which_keys_are_small(pkg, new, heads, kv, dim, large, n):
+    """One channel of q is `large` times the others, the keys are 0 on it (or one code for a few): the other channels
+    decide the scores and have to keep their bits."""
+    s = Setup(pkg, [new] * 12, [n] * 12, kv, dim, 16, seed=int(large) + new)
+    q = torch.randn(s.rows, heads * dim, device=dev(), generator=s.g)
+    q.view(s.rows, heads, dim)[:, :, 7] *= large
+    s.cache.keys[..., 7] = 0
+    for b in range(6):
+        page, slot = s.where(b)
+        s.cache.keys[page[1::3], :, slot[1::3], 7] = 1
+    want, tol = exact(s, q, heads, 1 / math.sqrt(dim))
+    compare(run(s, q, None), want, tol, s.rows)

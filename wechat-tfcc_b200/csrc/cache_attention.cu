@@ -35,14 +35,16 @@ namespace {
 // CTA barrier in the loop) and multiplies with mma.sync, whose fragments are read straight from
 // the rows as they lie because the order of k is free: a lane's 16 bytes of a key row serve as its k slots of
 // successive steps.
-//   Scores: q is a 24-bit integer per element (scaled by a power of two per row) in three balanced
+//   Scores: q is a 31-bit integer per element (scaled by a power of two per row) in four balanced
 //   8-bit digits, and the codes are multiplied as they are, m16n8k32 in integers: exact sums and no conversion of
-//   K at all.  With 8 rows two digits fill the 16 rows of one product, the third a second one.
+//   K at all.  Elements down to 2^-6 of the row's largest are held exactly, smaller ones to 2^-30 of it: with
+//   three digits (2^-22) a head with one large channel lost what the others say.  With 8 rows
+//   two digits fill the 16 rows of one product.
 //   Output: V becomes fp16 (1.5 instructions a code), weights as above; with 8 rows the 16 rows of
 //   m16n8k16 hold their hi and lo terms side by side.
 // Eight warps take the eight 16-key groups of a 128-key block and are added at the item's end.
-// Two sequences of 65536 keys, 64 / 8 heads of 128: 69 us, 4.0 TB/s, 0.61 of the measured copy rate; 32 ragged
-// ones, 32 / 8 heads: 74 us.  Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is
+// Two sequences of 65536 keys, 64 / 8 heads of 128: 68 us, 4.1 TB/s, 0.62 of the measured copy rate; 32 ragged
+// ones, 32 / 8 heads: 72 us; 24 ragged ones with 3 or 4 new tokens (16 rows): 111 us, 104 with three digits.  Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is
 // left is 4 us until the first loads, CTAs that finish 10 us apart, 4 us per item of a short sequence,
 // and the merge.  (Scores from fp16 terms of q instead of digits 83 us; three CTAs per SM with 80 registers
 // 126 us, because of spills.)
@@ -55,7 +57,7 @@ struct FewLayout {
   static constexpr int kCodeBytes = 16 * DIM;               // codes of 16 keys (or values)
   static constexpr int kStageBytes = 2 * kCodeBytes + 128;  // + their scales
   static constexpr int kRingBytes = kStages * kStageBytes;  // per warp
-  static constexpr int kFragBytes = (DIM / 32) * 32 * (ROWS == 8 ? 16 + 8 : 3 * 16);  // digits of q
+  static constexpr int kFragBytes = (DIM / 32) * 32 * (ROWS == 8 ? 2 : 4) * 16;  // digits of q
   static constexpr int kSmall = kFragBytes + kFewWarps * kRingBytes;
   static constexpr int kSmem = kSmall + kFewWarps * 3 * ROWS * 4;
   static_assert(ROWS * DIM * 4 <= kRingBytes, "a warp's sums reuse its ring");
@@ -80,17 +82,21 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint4 a, uint32_t b0, uint32
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// Four 24-bit integers -> three words of their balanced base-256 digits, lowest first.
-__device__ __forceinline__ void digits4(const int (&v)[4], uint32_t (&d)[3]) {
-  uint32_t x[4][3];
+// Four integers below 2^30 -> four words of their balanced base-256 digits, lowest first.
+__device__ __forceinline__ void digits4(const int (&v)[4], uint32_t (&d)[4]) {
+  uint32_t x[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int d0 = static_cast<int8_t>(v[i]), r1 = (v[i] - d0) >> 8;
-    const int d1 = static_cast<int8_t>(r1), d2 = (r1 - d1) >> 8;
-    x[i][0] = d0 & 0xff; x[i][1] = d1 & 0xff; x[i][2] = d2 & 0xff;
+    int r = v[i];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int low = static_cast<int8_t>(r);
+      x[i][k] = low & 0xff;
+      r = (r - low) >> 8;
+    }
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) d[k] = x[0][k] | (x[1][k] << 8) | (x[2][k] << 16) | (x[3][k] << 24);
+  for (int k = 0; k < 4; ++k) d[k] = x[0][k] | (x[1][k] << 8) | (x[2][k] << 16) | (x[3][k] << 24);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint4 a, uint32_t b0, uint32_t b1) {
@@ -262,16 +268,16 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       }
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      // 2^(21 - exponent): the row's largest value lands in [2^21, 2^22), inside three balanced digits.  Zero and
-      // tiny rows (below 2^-100) take the bound of the range; a row with an infinity or a NaN is NaN.
+      // 2^(29 - exponent): the row's largest value lands in [2^29, 2^30), inside four balanced digits.  Zero and
+      // tiny rows (below 2^-97) take the bound of the range; a row with an infinity or a NaN is NaN.
       const int ex = static_cast<int>(m >> 23) - 127;
-      const int sh = ex == 128 ? 0 : 21 - max(ex, -100);
+      const int sh = ex == 128 ? 0 : 29 - max(ex, -97);
       const float up = __uint_as_float(static_cast<uint32_t>(sh + 127) << 23);
       row_scale[h] = ex == 128 ? __uint_as_float(0x7fffffffu) : __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s % kFewWarps != static_cast<int>(warp) % kSteps) continue;
-        uint32_t d[2][3];
+        uint32_t d[2][4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float4 x = f[2 * s + e];
@@ -279,11 +285,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
           digits4(v, d[e]);
         }
         if constexpr (ROWS == 8) {
-          frag[s * 32 + lane] = make_uint4(d[0][2], d[0][1], d[1][2], d[1][1]);
-          reinterpret_cast<uint2*>(frag + kSteps * 32)[s * 32 + lane] = make_uint2(d[0][0], d[1][0]);
+          frag[s * 32 + lane] = make_uint4(d[0][3], d[0][2], d[1][3], d[1][2]);
+          frag[(kSteps + s) * 32 + lane] = make_uint4(d[0][1], d[0][0], d[1][1], d[1][0]);
         } else {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
+          for (int k = 0; k < 4; ++k) {
             uint32_t* w = reinterpret_cast<uint32_t*>(frag + (k * kSteps + s) * 32 + lane);
             w[h] = d[0][k];
             w[2 + h] = d[1][k];
@@ -322,9 +328,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
       // scores of keys 0-7 and 8-15 of the group: [2 j + e] of a lane (g, t) are keys 2 t + e (+ 8 j)
       float x[ROWS / 8][4];
       {
-        int c[ROWS == 8 ? 2 : 3][2][4];
+        constexpr int kProducts = ROWS == 8 ? 2 : 4;
+        int c[kProducts][2][4];
 #pragma unroll
-        for (int k = 0; k < (ROWS == 8 ? 2 : 3); ++k)
+        for (int k = 0; k < kProducts; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i) c[k][0][i] = c[k][1][i] = 0;
 #pragma unroll
@@ -335,36 +342,26 @@ __global__ void __launch_bounds__(kFewThreads, 2) cache_attention_few_kernel(con
           for (int e = 0; e < 2; ++e) {
             const int s = 2 * q + e;
             const uint32_t a0 = e ? ka.z : ka.x, a1 = e ? ka.w : ka.y, b0 = e ? kb.z : kb.x, b1 = e ? kb.w : kb.y;
-            if constexpr (ROWS == 8) {
-              const uint4 f = frag[s * 32 + lane];
-              const uint2 l = reinterpret_cast<const uint2*>(frag + kSteps * 32)[s * 32 + lane];
-              const uint4 fl = make_uint4(l.x, 0u, l.y, 0u);
-              mma_s8(c[0][0], f, a0, a1);
-              mma_s8(c[0][1], f, b0, b1);
-              mma_s8(c[1][0], fl, a0, a1);
-              mma_s8(c[1][1], fl, b0, b1);
-            } else {
 #pragma unroll
-              for (int k = 0; k < 3; ++k) {
-                const uint4 f = frag[(k * kSteps + s) * 32 + lane];
-                mma_s8(c[k][0], f, a0, a1);
-                mma_s8(c[k][1], f, b0, b1);
-              }
+            for (int k = 0; k < kProducts; ++k) {
+              const uint4 f = frag[(k * kSteps + s) * 32 + lane];
+              mma_s8(c[k][0], f, a0, a1);
+              mma_s8(c[k][1], f, b0, b1);
             }
           }
         }
-        // high digit * 2^16 + (middle * 2^8 + low): the bracket stays below 2^30
+        // (highest digit * 2^8 + next) * 2^16 + (third * 2^8 + lowest): the brackets stay below 2^30
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if constexpr (ROWS == 8) {
-              x[0][2 * j + e] = fmaf(static_cast<float>(c[0][j][e]), 65536.f,
-                                     static_cast<float>(c[0][j][2 + e] * 256 + c[1][j][e]));
+              x[0][2 * j + e] = fmaf(static_cast<float>(c[0][j][e] * 256 + c[0][j][2 + e]), 65536.f,
+                                     static_cast<float>(c[1][j][e] * 256 + c[1][j][2 + e]));
             } else {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                x[h][2 * j + e] = fmaf(static_cast<float>(c[2][j][2 * h + e]), 65536.f,
+                x[h][2 * j + e] = fmaf(static_cast<float>(c[3][j][2 * h + e] * 256 + c[2][j][2 * h + e]), 65536.f,
                                        static_cast<float>(c[1][j][2 * h + e] * 256 + c[0][j][2 * h + e]));
             }
           }
