@@ -551,7 +551,7 @@ TFCCB200_API int tfccb200_qgemm_u8s8s32_host(void* stream, const uint8_t* hA, un
  * and ld_codes are left as they are.
  *
  * tfccb200_qgemm_scaled_s8: C = act(a_scales[m] * b_scales[n] * (A.B)[m][n] + bias[n]), the int32
- * sums exact for K <= 133,000; A [M,K] s8 with rows lda apart, B [K,N] s8 with rows ldb apart, C [M,N]
+ * sums exact for any codes; K <= 131,071, so that they fit; A [M,K] s8 with rows lda apart, B [K,N] s8 with rows ldb apart, C [M,N]
  * fp32 dense, bias [N] or NULL.  Bases 16-byte aligned with lda and ldb multiples of 16 run on the tensor
  * cores (up to 16 tokens: a kernel that streams the weights, TFCCB200_PATH_SKINNY); any other layout on
  * the CUDA cores.  TFCCB200_EUNSUPPORTED when a forced path cannot take

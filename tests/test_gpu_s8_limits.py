@@ -1,0 +1,25 @@
+"""The 8-bit linear layer and the cache at the ends of their ranges, on the GPU."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+@pytest.mark.parametrize("m,path", [(1, "skinny"), (16, "auto"), (40, "umma"), (40, "umma2"), (40, "simt")])
+def test_the_largest_sums(pkg, m, path):
+    """K at its limit, codes of -128 in both operands: 2147467264, or its negative against 127.  One rounding of the
+    sum and two products with powers of two: within 2^-24."""
+    k = 131071
+    a = torch.full((m, k + 1), -128, dtype=torch.int8, device=dev())[:, :k]
+    b = torch.full((k, 32), -128, dtype=torch.int8, device=dev())
+    b[:, 16:] = 127
+    sa, sb = torch.full((m,), 0.5, device=dev()), torch.full((32,), 0.25, device=dev())
+    got = pkg.quantization.matmul_scaled(a, sa, b, sb, path=path).double()
+    want = torch.full_like(got, 128 * 128 * k / 8)
+    want[:, 16:] = -128 * 127 * k / 8
+    assert bool(((got - want).abs() <= 2.0 ** -24 * want.abs()).all())
+    pkg.session.get_session(dev()).sync()

@@ -1,0 +1,12 @@
+"""Limits of the 8-bit linear layer and the cache at the C entry points and in Python, without a GPU."""
+import pytest
+
+from test_s8_refusals import EOVERFLOW, P, linear_args
+
+
+@pytest.mark.parametrize("k", [131072, 132105, 133000])
+def test_sums_of_codes_of_minus_128_have_to_fit(pkg, k):
+    """128 * 128 * 131072 = 2^31."""
+    assert pkg.lib.tfccb200_qgemm_scaled_s8(*linear_args(K=k, lda=k // 16 * 16 + 16)) == EOVERFLOW
+    args = [None, P, k, P, 64, P, None, P, 2, 64, k, 0, P, 1 << 40, None]
+    assert pkg.lib.tfccb200_qlinear_f32(*args) == EOVERFLOW
