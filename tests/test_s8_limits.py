@@ -10,3 +10,9 @@ def test_sums_of_codes_of_minus_128_have_to_fit(pkg, k):
     assert pkg.lib.tfccb200_qgemm_scaled_s8(*linear_args(K=k, lda=k // 16 * 16 + 16)) == EOVERFLOW
     args = [None, P, k, P, 64, P, None, P, 2, 64, k, 0, P, 1 << 40, None]
     assert pkg.lib.tfccb200_qlinear_f32(*args) == EOVERFLOW
+
+
+@pytest.mark.parametrize("kw", [{"M": 1 << 31, "N": 1, "K": 1}, {"M": 0xffffffff, "N": 1, "K": 1}, {"M": 1, "N": 1 << 31, "K": 1, "ldb": 1 << 31}])
+@pytest.mark.parametrize("path", [0, 1, 3, 4])
+def test_rows_and_columns_that_a_tile_would_carry_past_32_bits(pkg, kw, path):
+    assert pkg.lib.tfccb200_qgemm_scaled_s8(*linear_args(**dict(kw, path=path))) == EOVERFLOW

@@ -841,7 +841,8 @@ int check_s8_gemm(const S8GemmArgs& a) {
   if (a.lda < a.K || a.ldb < a.N) return TFCCB200_EINVAL;
   if (a.activation != TFCCB200_ACT_NONE && a.activation != TFCCB200_ACT_GELU_ERF) return TFCCB200_EINVAL;
   if (a.K > 131071u) return TFCCB200_EOVERFLOW;  // 128 * 128 * K must fit an int32: codes may be -128
-  if (shape_overflows(a.M, a.N, a.K, 1)) return TFCCB200_EOVERFLOW;
+  // (the kernels add a tile's rows and columns to its first one in 32 bits, tensor maps count in signed ones)
+  if (a.M > 0x7fffffffu || a.N > 0x7fffffffu || shape_overflows(a.M, a.N, a.K, 1)) return TFCCB200_EOVERFLOW;
   if (misaligned(a.C, 4) || misaligned(a.a_scales, 4) || misaligned(a.b_scales, 4) || misaligned(a.bias, 4))
     return TFCCB200_EALIGN;
   return TFCCB200_OK;
