@@ -23,3 +23,20 @@ def test_the_largest_sums(pkg, m, path):
     want[:, 16:] = -128 * 127 * k / 8
     assert bool(((got - want).abs() <= 2.0 ** -24 * want.abs()).all())
     pkg.session.get_session(dev()).sync()
+
+
+@pytest.mark.parametrize("m,n,k", [(65536 * 64 + 3, 5, 3), (3, 65536 * 64 + 3, 2)])
+def test_operands_off_16_bytes_of_any_length(pkg, m, n, k):
+    """More tiles than a grid's second dimension has, on the CUDA-core path: nothing is refused, above all not after
+    the tokens have been quantized.  Results as from the same rows and columns in a small call."""
+    g = torch.Generator(device=dev()).manual_seed(1)
+    x = torch.randn(m, k, device=dev(), generator=g)
+    b = torch.randint(-127, 128, (k, n), device=dev(), generator=g).to(torch.int8)
+    s = torch.rand(n, device=dev(), generator=g)
+    got = pkg.quantization.linear(x, b, s)
+    codes, scales = pkg.quantization.quantize_tokens(x)
+    for rows, cols in ((slice(0, 70), slice(0, 5)), (slice(m - 70 if m > 70 else 0, m), slice(max(0, n - 5), n))):
+        sums = codes[rows].double() @ b[:, cols].double()
+        want = sums * scales[rows].double()[:, None] * s[cols].double()
+        assert bool(((got[rows, cols].double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all())
+    pkg.session.get_session(dev()).sync()

@@ -848,18 +848,41 @@ int check_s8_gemm(const S8GemmArgs& a) {
   return TFCCB200_OK;
 }
 
-int run_s8_gemm(const S8GemmArgs& a, int path) {
+// The path that takes the operands, or why none does (negative): everything that the product refuses by
+// itself, so that a caller can ask before it launches anything.
+int s8_gemm_path(const S8GemmArgs& a, int path) {
   const int st = check_s8_gemm(a);
   if (st != TFCCB200_OK) return st;
   switch (path) {
     case TFCCB200_PATH_AUTO:
-      if (few_s8_gemm_supported(a)) return few_s8_gemm(a);
-      return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, -1) : simt_s8_gemm(a);
-    case TFCCB200_PATH_SKINNY: return few_s8_gemm_supported(a) ? few_s8_gemm(a) : TFCCB200_EUNSUPPORTED;
-    case TFCCB200_PATH_SIMT: return simt_s8_gemm(a);
-    case TFCCB200_PATH_UMMA: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 0) : TFCCB200_EUNSUPPORTED;
-    case TFCCB200_PATH_UMMA2: return umma_s8_gemm_supported(a) ? umma_s8_gemm(a, 1) : TFCCB200_EUNSUPPORTED;
+      path = few_s8_gemm_supported(a) ? TFCCB200_PATH_SKINNY : umma_s8_gemm_supported(a) ? TFCCB200_PATH_UMMA : TFCCB200_PATH_SIMT;
+      break;
+    case TFCCB200_PATH_SIMT: break;
+    case TFCCB200_PATH_SKINNY:
+      if (!few_s8_gemm_supported(a)) return TFCCB200_EUNSUPPORTED;
+      break;
+    case TFCCB200_PATH_UMMA:
+    case TFCCB200_PATH_UMMA2:
+      if (!umma_s8_gemm_supported(a)) return TFCCB200_EUNSUPPORTED;
+      break;
     default: return TFCCB200_EINVAL;
+  }
+  if (path == TFCCB200_PATH_UMMA || path == TFCCB200_PATH_UMMA2) {
+    cudaError_t ce;
+    const DeviceInfo* di = current_device_info(&ce);
+    if (di && di->cc_major != 10) return TFCCB200_EUNSUPPORTED;  // (no device: the launch reports it)
+  }
+  return path;
+}
+
+int run_s8_gemm(const S8GemmArgs& a, int wanted) {
+  const int path = s8_gemm_path(a, wanted);
+  switch (path) {
+    case TFCCB200_PATH_SKINNY: return few_s8_gemm(a);
+    case TFCCB200_PATH_SIMT: return simt_s8_gemm(a);
+    case TFCCB200_PATH_UMMA: return umma_s8_gemm(a, wanted == TFCCB200_PATH_AUTO ? -1 : 0);
+    case TFCCB200_PATH_UMMA2: return umma_s8_gemm(a, 1);
+    default: return path;
   }
 }
 
@@ -941,9 +964,9 @@ int tfccb200_qlinear_f32(void* stream, const float* x, size_t ldx, const int8_t*
   a.M = M; a.N = N; a.K = K;
   a.activation = activation;
   a.status = device_status;
-  int st = check_s8_gemm(a);  // what the product would refuse is refused before the first launch
-  if (st != TFCCB200_OK) return st;
-  st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
+  const int path = s8_gemm_path(a, TFCCB200_PATH_AUTO);  // what the product would refuse is refused before the first launch
+  if (path < 0) return path;
+  const int st = tfccb200_quantize_tokens_f32(stream, x, ldx, M, K, const_cast<int8_t*>(a.A), a.lda, scales);
   a.early_weights = true;
   return st != TFCCB200_OK ? st : run_s8_gemm(a, TFCCB200_PATH_AUTO);
 }

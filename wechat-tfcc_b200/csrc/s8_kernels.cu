@@ -260,13 +260,15 @@ s8_few_kernel(const __grid_constant__ S8GemmArgs a, unsigned splits) {
   }
 }
 
-// Any pitch, any alignment: 64 x 64 results per CTA, 4 x 4 per thread, int32 sums.
+// Any pitch, any alignment: 64 x 64 results per CTA, 4 x 4 per thread, int32 sums.  Tiles along one grid dimension, so
+// that neither M nor N meets the bound of the others.
 __global__ void __launch_bounds__(256) s8_gemm_simt_kernel(const S8GemmArgs a) {
   constexpr int T = 64, KB = 32;
   __shared__ int8_t sa[KB][T + 4], sb[KB][T + 4];
   pdl_release();
   pdl_wait();
-  const unsigned m0 = blockIdx.y * T, n0 = blockIdx.x * T;
+  const unsigned across = (a.N - 1) / T + 1;
+  const unsigned m0 = blockIdx.x / across * T, n0 = blockIdx.x % across * T;
   const unsigned tx = threadIdx.x & 15u, ty = threadIdx.x >> 4;
   int acc[4][4] = {};
   for (unsigned k0 = 0; k0 < a.K; k0 += KB) {
@@ -368,8 +370,8 @@ int few_s8_gemm(const S8GemmArgs& a) {
 }
 
 int simt_s8_gemm(const S8GemmArgs& a) {
-  const dim3 grid((a.N + 63) / 64, (a.M + 63) / 64);
-  if (grid.y > 65535u) return TFCCB200_EUNSUPPORTED;
+  // (M * N fits 32 bits, M and N 31: fewer than 2^27 tiles)
+  const dim3 grid(((a.N - 1) / 64 + 1) * ((a.M - 1) / 64 + 1));
   cudaError_t e = launch_after_previous(s8_gemm_simt_kernel, grid, dim3(256), 0, a.stream, a);
   if (e != cudaSuccess) return static_cast<int>(e);
   count_launch();

@@ -725,8 +725,9 @@ int umma_qgemm(const QgemmArgs& a, bool pair) {
 
 bool umma_s8_gemm_supported(const S8GemmArgs& a) {
   // K and N may be anything: the tensor maps know them, and the pitches are what TMA wants to be
-  // multiples of 16 bytes.
-  return a.lda % 16 == 0 && a.ldb % 16 == 0 && aligned16(a.A) && aligned16(a.B);
+  // multiples of 16 bytes (and a matrix to be less than 2^40 bytes from end to end).
+  return a.lda % 16 == 0 && a.ldb % 16 == 0 && aligned16(a.A) && aligned16(a.B) &&
+         a.lda < (1ull << 40) / a.M && a.ldb < (1ull << 40) / a.K;
 }
 
 int umma_s8_gemm(const S8GemmArgs& a, int force_pair) {
