@@ -601,8 +601,8 @@ TFCCB200_API size_t tfccb200_qlinear_workspace(unsigned M, unsigned K);
  * tfccb200_cache_attention_f32: out_i = sum_j softmax_j(scale * q_i.k_j) v_j for q and out
  * [rows, heads * dim], query head h reading kv head h / (heads / kv_heads), j over the cached tokens
  * of the row's sequence up to its own position (causal) or all of them; a row that sees none is
- * 0.  max_new and max_length bound the new and cached tokens of one sequence; the launch is shaped
- * by them, and a sequence that exceeds them is passed over with TFCCB200_DEV_BAD_SEQUENCE.
+ * 0.  max_new and max_length bound the new and cached tokens of one sequence (larger ones than rows
+ * and table_width * page_size count as these); the launch is shaped by them, and a sequence that exceeds them is passed over with TFCCB200_DEV_BAD_SEQUENCE.
  * (max_new * heads / kv_heads / 128 + 1) * (max_length / 128 + 4) has to fit 32 bits.  starts, lengths
  * and table must not change while a call runs.
  * workspace: tfccb200_cache_attention_workspace bytes, 256-byte aligned.

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_gpu_cache import Setup
+
 pytestmark = pytest.mark.gpu
 
 
@@ -40,3 +42,27 @@ def test_operands_off_16_bytes_of_any_length(pkg, m, n, k):
         want = sums * scales[rows].double()[:, None] * s[cols].double()
         assert bool(((got[rows, cols].double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all())
     pkg.session.get_session(dev()).sync()
+
+
+@pytest.mark.parametrize("news,lengths,heads", [([1, 1], [3000, 700], 1), ([1], [9000], 8), ([60, 1], [700, 2000], 2)])
+def test_bounds_beyond_the_tensors_shape_the_launch_like_the_tensors(pkg, news, lengths, heads):
+    """UINT_MAX for "no bound" at the C entry: same kernels, same cuts, same bits as with the tensors' own extents."""
+    s = Setup(pkg, news, lengths, 1, 64, 16, seed=5)
+    q = torch.randn(s.rows, heads * 64, device=dev(), generator=s.g)
+    capacity = s.table.shape[1] * 16
+    scratch = torch.empty(64 << 20, dtype=torch.uint8, device=dev())
+    outs, launches = [], []
+    for most, longest in ((s.rows, capacity), (2 ** 32 - 1, capacity), (s.rows, 2 ** 32 - 1), (2 ** 32 - 1, 2 ** 32 - 100), (2 ** 31, 2 ** 31)):
+        need = pkg.lib.tfccb200_cache_attention_workspace(s.cache._ref, len(news), s.rows, heads, most, longest)
+        assert 0 < need <= scratch.numel()
+        out = torch.full_like(q, -1.0)
+        before = pkg.launch_count()
+        st = pkg.lib.tfccb200_cache_attention_f32(
+            torch.cuda.current_stream().cuda_stream, s.cache._ref, q.data_ptr(), q.shape[1], out.data_ptr(), q.shape[1], s.starts.data_ptr(),
+            s.lens.data_ptr(), s.table.data_ptr(), len(news), s.table.shape[1], s.rows, heads, most, longest, 0.125, 1, scratch.data_ptr(), need, None)
+        assert st == 0
+        outs.append(out)
+        launches.append(pkg.launch_count() - before)
+    assert len(set(launches)) == 1
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])

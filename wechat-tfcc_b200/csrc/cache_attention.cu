@@ -632,8 +632,8 @@ int cache_attention(const CacheAttentionArgs& args) {
   a.c = cache_params(args.cache);
   a.q = args.q; a.out = args.out; a.ldq = args.ldq; a.ldo = args.ldo;
   a.heads = args.heads; a.group = args.heads / args.cache.kv_heads;
-  if (args.max_new < a.c.max_new) a.c.max_new = args.max_new;
-  if (args.max_length < a.c.max_length) a.c.max_length = args.max_length;
+  a.c.max_new = args.max_new;
+  a.c.max_length = args.max_length;
   a.causal = args.causal;
   a.scale = args.scale * 1.4426950408889634f;
   a.scratch = args.max_length > kBlockKeys ? static_cast<float*>(args.workspace) : nullptr;

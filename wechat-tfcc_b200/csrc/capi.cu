@@ -999,7 +999,7 @@ size_t tfccb200_cache_attention_workspace(const tfccb200_cache* cache, unsigned 
   CacheAttentionArgs a = {};
   a.cache.kv_heads = cache->kv_heads; a.cache.dim = cache->dim; a.cache.page_size = cache->page_size;
   a.cache.batch = batch; a.cache.rows = rows;
-  a.heads = heads; a.max_new = max_new; a.max_length = max_length;
+  a.heads = heads; a.max_new = std::min(max_new, rows); a.max_length = max_length;
   return cache_attention_workspace(a);
 }
 
@@ -1015,15 +1015,17 @@ int tfccb200_cache_attention_f32(void* stream, const tfccb200_cache* cache, cons
   const size_t width = static_cast<size_t>(heads) * a.cache.dim;
   if ((st = check_rows(q, ldq, width)) != TFCCB200_OK || (st = check_rows(out, ldo, width)) != TFCCB200_OK) return st;
   if (static_cast<unsigned long long>(rows) * heads > 0x7fffffffull) return TFCCB200_EOVERFLOW;
+  // bounds beyond the tensors say nothing: launches are shaped by what the tensors can hold
+  max_new = std::min(max_new, rows);
+  max_length = static_cast<unsigned>(std::min<unsigned long long>(max_length, static_cast<unsigned long long>(table_width) * a.cache.page_size));
   a.q = q; a.out = out; a.ldq = ldq; a.ldo = ldo;
   a.heads = heads;
   a.max_new = max_new; a.max_length = max_length;
   a.scale = scale;
   a.causal = causal ? 1 : 0;
   // the kernels count a kv head's blocks of one sequence in 32 bits
-  const unsigned long long head_rows = static_cast<unsigned long long>(std::min(max_new, rows)) * (heads / a.cache.kv_heads);
-  const unsigned long long length = std::min<unsigned long long>(max_length, static_cast<unsigned long long>(table_width) * a.cache.page_size);
-  if ((head_rows / 128 + 1) * (length / 128 + 4) > 0xffffffffull) return TFCCB200_EOVERFLOW;
+  const unsigned long long head_rows = static_cast<unsigned long long>(max_new) * (heads / a.cache.kv_heads);
+  if ((head_rows / 128 + 1) * (max_length / 128 + 4ull) > 0xffffffffull) return TFCCB200_EOVERFLOW;
   a.workspace = workspace; a.workspace_bytes = workspace_bytes;
   const size_t need = cache_attention_workspace(a);
   if (need && (!workspace || misaligned(workspace, 256) || workspace_bytes < need)) return TFCCB200_EWORKSPACE;

@@ -256,7 +256,7 @@ struct CacheAttentionArgs {
   float* out;
   unsigned long long ldq, ldo;
   unsigned heads;
-  unsigned max_new, max_length;  // bounds the caller knows on the host
+  unsigned max_new, max_length;  // bounds the caller knows on the host, within rows and the table's capacity
   float scale;
   int causal;
   void* workspace;
