@@ -16,3 +16,14 @@ def test_sums_of_codes_of_minus_128_have_to_fit(pkg, k):
 @pytest.mark.parametrize("path", [0, 1, 3, 4])
 def test_rows_and_columns_that_a_tile_would_carry_past_32_bits(pkg, kw, path):
     assert pkg.lib.tfccb200_qgemm_scaled_s8(*linear_args(**dict(kw, path=path))) == EOVERFLOW
+
+
+def test_the_attributes_of_a_cache_are_fixed(pkg):
+    """Calls go by the addresses that the constructor took: a tensor put in another's place would leave them pointing
+    into freed memory."""
+    cache = pkg.cache.PagedCache.__new__(pkg.cache.PagedCache)
+    for name in ("keys", "key_scales", "values", "value_scales", "pages", "kv_heads", "page_size", "dim", "device"):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(cache, name, None)
+        with pytest.raises(AttributeError, match="fixed"):
+            delattr(cache, name)

@@ -35,7 +35,10 @@ class _Struct(C.Structure):  # tfccb200_cache of include/tfcc_b200.h
 class PagedCache:
     """The pool: ``keys`` / ``values`` int8 ``[pages, kv_heads, page_size, dim]``, ``key_scales`` /
     ``value_scales`` float32 ``[pages, kv_heads, page_size]``, all contiguous on one CUDA device.
-    ``dim`` is 64 or 128, ``page_size`` a power of two up to 1024."""
+    ``dim`` is 64 or 128, ``page_size`` a power of two up to 1024.
+
+    The attributes are fixed: calls go by the addresses taken here, so another tensor needs another
+    ``PagedCache`` (the tensors' contents are the caller's to change)."""
 
     __slots__ = ("keys", "key_scales", "values", "value_scales", "pages", "kv_heads", "page_size", "dim",
                  "device", "_struct", "_ref")
@@ -55,16 +58,26 @@ class PagedCache:
         for t in (keys, key_scales, values, value_scales):
             if not t.is_cuda or t.get_device() != device.index or not t.is_contiguous():
                 raise exceptions.InvalidArgumentError("the cache's tensors must be contiguous CUDA tensors on one device")
-        self.pages, self.kv_heads, self.page_size, self.dim = shape
-        if self.dim not in (64, 128):
-            raise exceptions.InvalidArgumentError(f"the cache exists for dim 64 and 128, not {self.dim}")
-        if self.page_size > 1024 or self.page_size & (self.page_size - 1):
-            raise exceptions.InvalidArgumentError(f"page_size must be a power of two up to 1024, not {self.page_size}")
-        self.keys, self.key_scales, self.values, self.value_scales = keys, key_scales, values, value_scales
-        self.device = device
-        self._struct = _Struct(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(),
-                               self.pages, self.page_size, self.kv_heads, self.dim)
-        self._ref = C.byref(self._struct)
+        pages, kv_heads, page_size, dim = shape
+        if dim not in (64, 128):
+            raise exceptions.InvalidArgumentError(f"the cache exists for dim 64 and 128, not {dim}")
+        if page_size > 1024 or page_size & (page_size - 1):
+            raise exceptions.InvalidArgumentError(f"page_size must be a power of two up to 1024, not {page_size}")
+        struct = _Struct(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(),
+                         pages, page_size, kv_heads, dim)
+        fixed = object.__setattr__
+        for name, value in (("keys", keys), ("key_scales", key_scales), ("values", values), ("value_scales", value_scales),
+                            ("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("dim", dim),
+                            ("device", device), ("_struct", struct), ("_ref", C.byref(struct))):
+            fixed(self, name, value)
+
+    def __setattr__(self, name, value):
+        if value is not None and getattr(self, name, None) is value:
+            return  # ``cache.keys *= 2`` works in place and puts the same tensor back
+        raise AttributeError(f"{name} of a PagedCache is fixed: make another one")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{name} of a PagedCache is fixed")
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, device) -> "PagedCache":
