@@ -18,6 +18,7 @@ The reference has no cache; its attention block is a graph of matmuls over whole
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import torch
 
@@ -32,6 +33,21 @@ class _Struct(C.Structure):  # tfccb200_cache of include/tfcc_b200.h
                 ("kv_heads", C.c_uint), ("dim", C.c_uint)]
 
 
+def _fixed(name):
+    """An attribute that is read, and set to nothing but what it is (``cache.keys *= 2`` works in place and puts the
+    same tensor back)."""
+    slot = "_" + name
+
+    def put(self, value):
+        if value is None or getattr(self, slot, None) is not value:
+            raise AttributeError(f"{name} of a PagedCache is fixed: make another one")
+
+    def drop(self):
+        raise AttributeError(f"{name} of a PagedCache is fixed")
+
+    return property(operator.attrgetter(slot), put, drop)
+
+
 class PagedCache:
     """The pool: ``keys`` / ``values`` int8 ``[pages, kv_heads, page_size, dim]``, ``key_scales`` /
     ``value_scales`` float32 ``[pages, kv_heads, page_size]``, all contiguous on one CUDA device.
@@ -40,8 +56,11 @@ class PagedCache:
     The attributes are fixed: calls go by the addresses taken here, so another tensor needs another
     ``PagedCache`` (the tensors' contents are the caller's to change)."""
 
-    __slots__ = ("keys", "key_scales", "values", "value_scales", "pages", "kv_heads", "page_size", "dim",
-                 "device", "_struct", "_ref")
+    __slots__ = ("_keys", "_key_scales", "_values", "_value_scales", "_pages", "_kv_heads", "_page_size", "_dim",
+                 "_device", "_struct", "_ref")
+    keys, key_scales, values, value_scales = _fixed("keys"), _fixed("key_scales"), _fixed("values"), _fixed("value_scales")
+    pages, kv_heads, page_size, dim = _fixed("pages"), _fixed("kv_heads"), _fixed("page_size"), _fixed("dim")
+    device = _fixed("device")
 
     def __init__(self, keys: torch.Tensor, key_scales: torch.Tensor, values: torch.Tensor,
                  value_scales: torch.Tensor):
@@ -63,21 +82,11 @@ class PagedCache:
             raise exceptions.InvalidArgumentError(f"the cache exists for dim 64 and 128, not {dim}")
         if page_size > 1024 or page_size & (page_size - 1):
             raise exceptions.InvalidArgumentError(f"page_size must be a power of two up to 1024, not {page_size}")
-        struct = _Struct(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(),
-                         pages, page_size, kv_heads, dim)
-        fixed = object.__setattr__
-        for name, value in (("keys", keys), ("key_scales", key_scales), ("values", values), ("value_scales", value_scales),
-                            ("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("dim", dim),
-                            ("device", device), ("_struct", struct), ("_ref", C.byref(struct))):
-            fixed(self, name, value)
-
-    def __setattr__(self, name, value):
-        if value is not None and getattr(self, name, None) is value:
-            return  # ``cache.keys *= 2`` works in place and puts the same tensor back
-        raise AttributeError(f"{name} of a PagedCache is fixed: make another one")
-
-    def __delattr__(self, name):
-        raise AttributeError(f"{name} of a PagedCache is fixed")
+        self._keys, self._key_scales, self._values, self._value_scales = keys, key_scales, values, value_scales
+        self._pages, self._kv_heads, self._page_size, self._dim, self._device = pages, kv_heads, page_size, dim, device
+        self._struct = _Struct(keys.data_ptr(), key_scales.data_ptr(), values.data_ptr(), value_scales.data_ptr(),
+                               pages, page_size, kv_heads, dim)
+        self._ref = C.byref(self._struct)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, device) -> "PagedCache":
@@ -92,12 +101,12 @@ def _sequences(cache, starts, lengths, table):
     """(starts, lengths, table pointers, batch, table width) of a call, checked."""
     if not isinstance(cache, PagedCache):
         raise exceptions.InvalidArgumentError("cache must be a PagedCache")
-    index = cache.device.index
+    index = cache._device.index
     for t, name, rank in ((starts, "starts", 1), (lengths, "lengths", 1), (table, "table", 2)):
         # (a tensor of the CPU has device -1)
         if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != index or \
                 len(t.shape) != rank or 0 in t.shape or not t.is_contiguous():
-            raise exceptions.InvalidArgumentError(f"{name}: expected a contiguous int32 tensor of rank {rank} on {cache.device}")
+            raise exceptions.InvalidArgumentError(f"{name}: expected a contiguous int32 tensor of rank {rank} on {cache._device}")
     batch, width = table.shape
     if lengths.shape[0] != batch or starts.shape[0] != batch + 1:
         raise exceptions.InvalidArgumentError("starts, lengths and table don't match")
@@ -123,10 +132,10 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, starts: torch.Te
     a packed projection will do) into their pages, one scale per token and head by the rule of
     ``quantization.quantize_tokens``.  No two new tokens may share a slot."""
     ps, pl, pt, batch, width = _sequences(cache, starts, lengths, table)
-    cols = cache.kv_heads * cache.dim
-    ldk = _packed(k, "k", None, cols, cache.device)
-    ldv = _packed(v, "v", k.shape[0], cols, cache.device)
-    sess, stream, guard = launch_context(cache.device)
+    cols = cache._kv_heads * cache._dim
+    ldk = _packed(k, "k", None, cols, cache._device)
+    ldv = _packed(v, "v", k.shape[0], cols, cache._device)
+    sess, stream, guard = launch_context(cache._device)
     with guard:
         check(lib.tfccb200_cache_append_f32(stream, cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv,
                                             ps, pl, pt, batch, width, k.shape[0], sess.status_ptr))
@@ -139,17 +148,17 @@ def read(cache: PagedCache, starts: torch.Tensor, lengths: torch.Tensor, table: 
     (``starts[b+1] - starts[b] == lengths[b]``) it reads all of them.  Rows behind ``starts[batch]``
     are left as they are in ``out`` (uninitialised when there is none)."""
     ps, pl, pt, batch, width = _sequences(cache, starts, lengths, table)
-    cols = cache.kv_heads * cache.dim
+    cols = cache._kv_heads * cache._dim
     if out is None:
         if rows <= 0:
             raise exceptions.InvalidArgumentError("rows must be positive")
-        k, v = cache.key_scales.new_empty((rows, cols)), cache.key_scales.new_empty((rows, cols))
+        k, v = cache._key_scales.new_empty((rows, cols)), cache._key_scales.new_empty((rows, cols))
         ldk = ldv = cols
     else:
         k, v = out
-        ldk = _packed(k, "out[0]", rows, cols, cache.device)
-        ldv = _packed(v, "out[1]", rows, cols, cache.device)
-    sess, stream, guard = launch_context(cache.device)
+        ldk = _packed(k, "out[0]", rows, cols, cache._device)
+        ldv = _packed(v, "out[1]", rows, cols, cache._device)
+    sess, stream, guard = launch_context(cache._device)
     with guard:
         check(lib.tfccb200_cache_read_f32(stream, cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv,
                                           ps, pl, pt, batch, width, rows, sess.status_ptr))
@@ -170,23 +179,23 @@ def attention(cache: PagedCache, q: torch.Tensor, starts: torch.Tensor, lengths:
     Rows behind ``starts[batch]`` are left as they are in ``out`` (uninitialised when there is none).
     """
     ps, pl, pt, batch, width = _sequences(cache, starts, lengths, table)
-    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (cache.kv_heads * cache.dim):
+    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (cache._kv_heads * cache._dim):
         raise exceptions.InvalidArgumentError("q: expected [rows, heads*dim] with heads a multiple of the cache's kv_heads")
     rows, cols = q.shape
-    ldq = _packed(q, "q", None, cols, cache.device)
+    ldq = _packed(q, "q", None, cols, cache._device)
     if out is None:
         out, ldo = q.new_empty((rows, cols)), cols
     else:
-        ldo = _packed(out, "out", rows, cols, cache.device)
+        ldo = _packed(out, "out", rows, cols, cache._device)
     max_new = rows if max_new is None else max_new
-    max_length = width * cache.page_size if max_length is None else max_length
+    max_length = width * cache._page_size if max_length is None else max_length
     if max_new <= 0 or max_length <= 0:
         raise exceptions.InvalidArgumentError("max_new and max_length must be positive")
-    max_new, max_length = min(max_new, rows), min(max_length, width * cache.page_size)
-    heads = cols // cache.dim
+    max_new, max_length = min(max_new, rows), min(max_length, width * cache._page_size)
+    heads = cols // cache._dim
     if scale is None:
-        scale = 1.0 / float(cache.dim) ** 0.5
-    sess, stream, guard = launch_context(cache.device)
+        scale = 1.0 / float(cache._dim) ** 0.5
+    sess, stream, guard = launch_context(cache._device)
     with guard:
         args = (stream, cache._ref, q.data_ptr(), ldq, out.data_ptr(), ldo, ps, pl, pt, batch, width, rows, heads,
                 max_new, max_length, float(scale), 1 if causal else 0)
