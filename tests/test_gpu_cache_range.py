@@ -138,6 +138,26 @@ def test_value_scales_spread_over_many_powers(pkg, new, dim):
     compare(run(s, q, None), want, tol, s.rows)
 
 
+@pytest.mark.parametrize("below", [14, 30, 50])
+@pytest.mark.parametrize("new,heads,kv,dim", [(1, 4, 1, 128), (16, 1, 1, 64), (200, 2, 1, 64), (150, 2, 2, 128), (2, 20, 1, 128)])
+def test_a_token_with_most_of_the_weight_and_no_values(pkg, new, heads, kv, dim, below):
+    """One token scores `below` above the others (in natural units, about), and its values are zeros: what is left of
+    the others is all of the result."""
+    n = 500
+    s = Setup(pkg, [new], [n], kv, dim, 32, seed=below + new)
+    q = torch.randn(new, heads * dim, device=dev(), generator=s.g)
+    q.view(new, heads, dim)[:, :, 0] = 8.0
+    page, slot = s.where(0)
+    for pos in (0, 270):
+        s.cache.keys[page[pos], :, slot[pos]] = 0
+        s.cache.keys[page[pos], :, slot[pos], 0] = 127
+        s.cache.key_scales[page[pos], :, slot[pos]] = below / 127
+        s.cache.values[page[pos], :, slot[pos]] = 0
+        s.cache.value_scales[page[pos], :, slot[pos]] = 0
+    want, tol = exact(s, q, heads, 0.125)
+    compare(run(s, q, 0.125), want, tol, new)
+
+
 @pytest.mark.parametrize("news,lengths", [([1, 1], [9000, 5000]), ([160], [6000])])
 def test_pieces_of_cut_items_with_scales_that_differ(pkg, news, lengths):
     """Long sequences, whose keys several CTAs share: each piece has a range of scales of its own."""

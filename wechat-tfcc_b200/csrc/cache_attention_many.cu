@@ -310,10 +310,11 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
           }
           top = __reduce_max_sync(0xffffffffu, top);
           top = min((top + 0x7fffffu) & 0x7f800000u, 0x7f000000u);  // up to a power of two
-          bool wide = false;  // a scale other than 0 lies 2^kValueRange below
+          bool wide = false;  // a key's scale lies 2^kValueRange below (0 does, whose key may have all the weight)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            wide |= (__float_as_uint(vs[i]) & 0x7fffffffu) - 1u < top - (static_cast<uint32_t>(kValueRange) << 23) - 1u;
+            wide |= static_cast<int>(blk * kBlockKeys + i * 32 + lane) < it.length &&
+                    (__float_as_uint(vs[i]) & 0x7fffffffu) < top - (static_cast<uint32_t>(kValueRange) << 23);
           wide = __any_sync(0xffffffffu, wide);
           // wide: scales as they are, or brought down so that exponentials relative to a weight have the range for it
           const float unit = !wide ? __uint_as_float(top) * (1.f / kWeightTop) : top > kWideTop ? kWideUnit : 1.f;
@@ -617,7 +618,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         return true;
       };
       // One block whose value scales spread wide.  A row's reference is the one that puts its largest weight at
-      // 2^13 (but no less than 2^-60 of its largest exponential, for the sum of these).  The scores are
+      // 2^13 (but no less than 2^-90 of its largest exponential, for the sum of these).  The scores are
       // read from tensor memory twice, 64 at a time: kept, they would cost the loop above registers.
       auto wide_block = [&](unsigned j) {
         const unsigned s = nb & 1u;
@@ -668,7 +669,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
             top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o2));
             ref[k] = fmaxf(ref[k], __shfl_xor_sync(0xffffffffu, ref[k], o2));
           }
-          ref[k] = fmaxf(ref[k] - 13.f, top[k] - 60.f);
+          ref[k] = fmaxf(ref[k] - 13.f, top[k] - 90.f);
           if (top[k] > m[k] + kLazy) {
             const float f = relative_to(m[k], top[k]);
             m[k] = top[k];
