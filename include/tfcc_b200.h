@@ -555,7 +555,8 @@ TFCCB200_API int tfccb200_qgemm_u8s8s32_host(void* stream, const uint8_t* hA, un
  * fp32 dense, bias [N] or NULL.  Bases 16-byte aligned with lda and ldb multiples of 16 run on the tensor
  * cores (up to 16 tokens: a kernel that streams the weights, TFCCB200_PATH_SKINNY); any other layout on
  * the CUDA cores.  TFCCB200_EUNSUPPORTED when a forced path cannot take
- * the operands.
+ * the operands.  GELU's erf is off by at most 1.5e-7 on the tensor cores (a rational approximation) and by erff's
+ * rounding on the other paths, so a token's last bits may depend on how many share the call.
  *
  * tfccb200_qlinear_f32: both in one call: x [M,K] fp32 with rows ldx apart, the codes and scales of x
  * in the caller's workspace (tfccb200_qlinear_workspace bytes, 256-byte aligned).
@@ -604,7 +605,9 @@ TFCCB200_API size_t tfccb200_qlinear_workspace(unsigned M, unsigned K);
  * 0.  max_new and max_length bound the new and cached tokens of one sequence (larger ones than rows
  * and table_width * page_size count as these); the launch is shaped by them, and a sequence that exceeds them is passed over with TFCCB200_DEV_BAD_SEQUENCE.
  * (max_new * heads / kv_heads / 128 + 1) * (max_length / 128 + 4) has to fit 32 bits.  starts, lengths
- * and table must not change while a call runs.
+ * and table must not change while a call runs.  Results are within about 2^-19 of the sum of |weight * value| of
+ * the keys that a row sees (scores within 2^-19 of sum |q k|, or 2^-30 max|q| sum |k| where that is more), whatever
+ * the other keys hold, and repeat bit by bit.
  * workspace: tfccb200_cache_attention_workspace bytes, 256-byte aligned.
  */
 typedef struct tfccb200_cache {

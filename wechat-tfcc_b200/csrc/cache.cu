@@ -7,7 +7,9 @@
 // one row (the sequence and page are looked up once for it) and walks the row's 2 * kv_heads
 // vectors, four per step with all their loads requested before the first is used; append asks for its first
 // values before it looks up where they go.  Bound by memory once there are rows enough: 16384 tokens of 8 x 128
-// written in 41 us (4.1 TB/s; 51 us with the look-up first), read back in 30 us (5.5 TB/s).
+// read back in 30 us (5.5 TB/s), written in 41 us (4.1 TB/s; 51 us with the look-up first): append asks for a
+// warp's next four vectors when the present ones have been quantized, into the same registers, and has no load in
+// flight meanwhile.
 #include <cuda_runtime.h>
 
 #include "cache.cuh"

@@ -44,9 +44,9 @@ namespace {
 //   m16n8k16 hold their hi and lo terms side by side.
 // Eight warps take the eight 16-key groups of a 128-key block and are added at the item's end.
 // Two sequences of 65536 keys, 64 / 8 heads of 128: 68 us, 4.1 TB/s, 0.62 of the measured copy rate; 32 ragged
-// ones, 32 / 8 heads: 72 us; 24 ragged ones with 3 or 4 new tokens (16 rows): 111 us, 104 with three digits.  Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is
-// left is 4 us until the first loads, CTAs that finish 10 us apart, 4 us per item of a short sequence,
-// and the merge.  (Scores from fp16 terms of q instead of digits 83 us; three CTAs per SM with 80 registers
+// ones, 32 / 8 heads: 72 us; 24 ragged ones with 3 or 4 new tokens (16 rows): 111 us, 104 with three digits.
+// Inside the loop a CTA pair reads 44 GB/s per SM, the copy rate; what is left is 4 us until the
+// first loads, CTAs that finish 10 us apart, 4 us per item of a short sequence, and the merge.  (Scores from fp16 terms of q instead of digits 83 us; three CTAs per SM with 80 registers
 // 126 us, because of spills.)
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -640,9 +640,11 @@ int cache_attention(const CacheAttentionArgs& args) {
   const bool wide = args.cache.dim == 128;
   int st = TFCCB200_OK;
   // Whether a sequence has few rows or many is device data.  Where max_new says that there may be both
-  // kinds, both kernels are launched, unless all blocks together are so few that the second kernel
-  // and its merge cost more (about 10 us) than the many-rows kernel loses on the others (1.4 us
-  // per block and SM).
+  // kinds, both kernels are launched, unless all blocks together are so few (7 per SM, the bound over all
+  // sequences) that the second kernel and its merge cost more than the many-rows kernel loses on the others.  Measured
+  // with 4 to 32 sequences of 1 to 24 new tokens, and with one chunk among single tokens: up to 7 blocks per SM
+  // 10 to 37 us in one kernel and 22 to 62 in two; they meet at 20 to 40 blocks per SM at dim 64 and at 50 or more at
+  // dim 128, so that the rule errs on the side of two kernels.
   const bool only_few = static_cast<unsigned long long>(args.max_new) * a.group <= kFewRows;
   const bool only_many = a.group > kFewRows || (!only_few && few_units_bound(args) * 14 <= 100ull * di->sm_count);
   if (!only_many) {

@@ -26,13 +26,13 @@
 //               and 64 sums fit the registers, a row's maximum and sum are two shuffles, and a
 //               thread reads the scales of 32 keys instead of 128
 // Bound by the tensor core: 8 dim flops per row and key instead of the 4 counted, at the rate the card
-// sustains on dense data.  4096 new tokens on 4096 cached ones, 32 / 8 heads of 128: 840 us, 491 TFLOP/s
-// counted, 982 executed (0.60 of the measured burst rate of bf16 products, 0.70 of the sustained one).  What was
+// sustains on dense data.  4096 new tokens on 4096 cached ones, 32 / 8 heads of 128: 843 us, 489 TFLOP/s
+// counted, 978 executed (0.60 of the measured burst rate of bf16 products, 0.70 of the sustained one).  What was
 // measured on the way there (the same case): a thread per row with all of its 128 sums, two
 // tiles per CTA 1137; two threads per row 1193; this layout 955; products issued with precomputed
 // descriptors 932; items weighted in the schedule 870; scales in the order of their reading 838.
 // Ordinary loads in place of read-only ones, pages looked up four at a time: 840.  References per block
-// and the path for value scales that spread wide: 833 to 844 (with that path in the registers of the main one 850 to
+// and the path for value scales that spread wide: 833 to 843 (with that path in the registers of the main one 850 to
 // 885).
 // Slower: sixteen softmax warps 1088, products summed over four blocks in tensor memory 972, codes
 // through a ring of bulk copies 880, code loads two tiles ahead 930,

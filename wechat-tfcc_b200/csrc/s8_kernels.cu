@@ -100,9 +100,13 @@ quantize_tokens_kernel(const float* src, unsigned long long ld_src, unsigned row
 // order: lane group g holds columns 16 g .. 16 g + 15, column j of each for the j-th product.  With
 // the tokens as rows the products cost 16 instructions per 4 KB of weights.  The int32 sums of the warps
 // meet in shared memory and those of a K split in the shared memory of a thread-block cluster;
-// integer sums are exact in any order.  (The tcgen05 kernel pads 16 tokens to 128 rows and
-// leaves its epilogue to one warp per tile: 43 us for 16x4096x16384 with GELU; two steps
-// held in registers instead of the ring: 21 us; this form 15 us, 4.5 TB/s of weights; six stages no faster.)
+// integer sums are exact in any order.  16x4096x16384 with GELU, weights from memory: 16.4 us, 4.1 TB/s.  The
+// tcgen05 kernel, which pads 16 tokens to 128 rows and leaves its epilogue to one warp per tile, takes 22.8; over
+// 4096 -> 11008, 4096 -> 16384 and 5120 -> 20480 it takes 21 to 37 us for 16 tokens and this one 15 to 34, which is why
+// this one goes up to the 16 rows of its product.  (Two steps held in registers instead of the ring: 21 us for
+// the first case; six stages no faster.)  What it leaves: whole 128-column tiles, and K split by powers of two only
+// while all CTAs fit, keep 128 of 148 SMs busy at N = 16384 (K in one piece) and 86 at 11008; at 20480 there are
+// 160 CTAs, two waves.
 constexpr int kFewThreads = 256;
 constexpr int kFewCols = 128;
 constexpr int kFewPitch = kFewCols + 12;  // ints per token in shared memory: rows start 12 banks apart
