@@ -631,6 +631,7 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
         float ref[2] = {-INFINITY, -INFINITY}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
         // scores 64 h .. of the block, -inf where a row does not see the key
         auto scores = [&](int h, uint32_t (&x)[32]) {
+          __syncwarp();  // accesses to tensor memory want the warp whole
           ptx::tmem_ld_16x64(t_s + 64 * h, x);
           ptx::tmem_ld_wait();
 #pragma unroll
@@ -670,9 +671,13 @@ cache_attention_many_kernel(const __grid_constant__ CacheAttention a, unsigned l
             ref[k] = fmaxf(ref[k], __shfl_xor_sync(0xffffffffu, ref[k], o2));
           }
           ref[k] = fmaxf(ref[k] - 13.f, top[k] - 90.f);
-          if (top[k] > m[k] + kLazy) {
-            const float f = relative_to(m[k], top[k]);
-            m[k] = top[k];
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float next = top[k] > m[k] + kLazy ? top[k] : m[k];
+            const float f = relative_to(m[k], next);
+            m[k] = next;
             l[k] *= f;
             back[k] *= f;
 #pragma unroll
